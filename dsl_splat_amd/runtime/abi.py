@@ -9,7 +9,7 @@ import ctypes
 c_float_p = ctypes.POINTER(ctypes.c_float)
 c_int32_p = ctypes.POINTER(ctypes.c_int32)
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 # Tile modes (GS3D_TILE_*), named as the reference's TileMode literals.
 TILE_MODES = {"radius": 0, "snugbox": 1, "accutile": 2}
@@ -20,6 +20,13 @@ GS3D_ERR_LAUNCH = -2
 GS3D_ERR_UNSUPPORTED = -3
 GS3D_ERR_SCRATCH = -4
 GS3D_ERR_OVERFLOW = -5
+# Feature decoder: element types, activations and limits (GS3D_F32 ..,
+# GS3D_ACT_.., GS3D_MAX_..).
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
+MAX_CHANNELS = 4096
+MAX_ROWS = 1 << 29
+MAX_IMAGES = 65535
 # Static scratch of gs3d_sort_pairs_u64_static (GS3D_STATIC_SCRATCH_BYTES).
 STATIC_SCRATCH_BYTES = 128 << 20
 
@@ -243,6 +250,85 @@ class RenderBwdArgs(ctypes.Structure):
     ]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("inner", ctypes.c_int32),
+        ("outer", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("x", _P),
+        ("x_stride", ctypes.c_int64),
+        ("weight", _P),
+        ("bias", _P),
+        ("residual", _P),
+        ("residual_stride", ctypes.c_int64),
+        ("y", _P),
+    ]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("inner", ctypes.c_int32),
+        ("outer", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("x", _P),
+        ("x_stride", ctypes.c_int64),
+        ("codes", _P),
+        ("scales", _P),
+        ("weight", _P),
+        ("bias", _P),
+        ("upstream", _P),
+        ("upstream_stride", ctypes.c_int64),
+        ("grad_x", _P),
+        ("grad_weight", _P),
+        ("grad_bias", _P),
+    ]
+
+
+class GroupNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("images", ctypes.c_int32),
+        ("pixels", ctypes.c_int64),
+        ("channels", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("x", _P),
+        ("x_stride", ctypes.c_int64),
+        ("weight", _P),
+        ("bias", _P),
+        ("y", _P),
+        ("statistics", _P),
+    ]
+
+
+class GroupNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("images", ctypes.c_int32),
+        ("pixels", ctypes.c_int64),
+        ("channels", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("x", _P),
+        ("x_stride", ctypes.c_int64),
+        ("codes", _P),
+        ("scales", _P),
+        ("weight", _P),
+        ("bias", _P),
+        ("statistics", _P),
+        ("upstream", _P),
+        ("upstream_stride", ctypes.c_int64),
+        ("grad_x", _P),
+        ("grad_weight", _P),
+        ("grad_bias", _P),
+    ]
+
+
 STRUCTS = {
     "gs3d_project_args": ProjectArgs,
     "gs3d_project_bwd_args": ProjectBwdArgs,
@@ -252,6 +338,10 @@ STRUCTS = {
     "gs3d_render_args": RenderArgs,
     "gs3d_render_stats_args": RenderStatsArgs,
     "gs3d_render_bwd_args": RenderBwdArgs,
+    "gs3d_linear_args": LinearArgs,
+    "gs3d_linear_bwd_args": LinearBwdArgs,
+    "gs3d_group_norm_args": GroupNormArgs,
+    "gs3d_group_norm_bwd_args": GroupNormBwdArgs,
 }
 
 # Exported functions: name -> (restype, argtypes).  void* carries device
@@ -307,4 +397,12 @@ FUNCTIONS = {
     "gs3d_render_fwd_stats": (ctypes.c_int, [ctypes.POINTER(RenderArgs), ctypes.POINTER(RenderStatsArgs), _P]),
     "gs3d_render_bwd": (ctypes.c_int, [ctypes.POINTER(RenderBwdArgs), _P]),
     "gs3d_render_bwd_lists": (ctypes.c_int, [ctypes.POINTER(RenderBwdArgs), _I64, _P]),
+    "gs3d_linear_fwd": (ctypes.c_int, [ctypes.POINTER(LinearArgs), _P]),
+    "gs3d_linear_bwd_scratch_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
+    "gs3d_linear_bwd": (ctypes.c_int, [ctypes.POINTER(LinearBwdArgs), _P, _SZ, _P]),
+    "gs3d_group_norm_scratch_bytes": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
+    "gs3d_group_norm_fwd": (ctypes.c_int, [ctypes.POINTER(GroupNormArgs), _P, _SZ, _P]),
+    "gs3d_group_norm_bwd": (ctypes.c_int, [ctypes.POINTER(GroupNormBwdArgs), _P, _SZ, _P]),
+    "gs3d_quantize_activations": (ctypes.c_int, [_P, _I64, _I64, _I32, _I32, _P, _P, _P]),
+    "gs3d_dequantize_activations": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _P, _P]),
 }

@@ -537,6 +537,128 @@ int gs3d_render_bwd(const gs3d_render_bwd_args* args, void* stream);
  * the launch shape of mid-size grids follows the entries per Gaussian. */
 int gs3d_render_bwd_lists(const gs3d_render_bwd_args* args, int64_t ids_count, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Feature-image decoder: the per-pixel network that turns rendered feature
+ * images (views,H,W,D) into the space they are trained in.  No counterpart
+ * in the reference, whose path ends at the images.
+ *
+ * Element types GS3D_F32 / GS3D_BF16 / GS3D_F16: activations, weights, biases
+ * and their gradients share one; sums, statistics and activations are held in
+ * 32 bits.  Rows (pixels) have contiguous channels and a row stride in
+ * elements; strided arguments say so, the others are contiguous.  No
+ * alignment beyond the element's own is required.
+ * ---------------------------------------------------------------------- */
+enum { GS3D_F32 = 0, GS3D_BF16 = 1, GS3D_F16 = 2 };
+
+/* act(z): z, max(z, 0), z sigmoid(z), z Phi(z) with Phi the normal
+ * distribution function. */
+enum { GS3D_ACT_NONE = 0, GS3D_ACT_RELU = 1, GS3D_ACT_SILU = 2, GS3D_ACT_GELU = 3 };
+
+#define GS3D_MAX_CHANNELS 4096
+#define GS3D_MAX_ROWS (1 << 29)     /* pixels of all images of a call */
+#define GS3D_MAX_IMAGES 65535
+
+/* y = act(x W^T + bias) + residual: x (rows, inner), W (outer, inner), y
+ * (rows, outer).  bias and residual may be NULL. */
+typedef struct gs3d_linear_args {
+    int64_t rows;
+    int32_t inner, outer;
+    int32_t dtype, activation;
+    const void* x;
+    int64_t x_stride;
+    const void* weight;
+    const void* bias;
+    const void* residual;
+    int64_t residual_stride;
+    void* y;
+} gs3d_linear_args;
+
+int gs3d_linear_fwd(const gs3d_linear_args* args, void* stream);
+
+/* Gradients of gs3d_linear_fwd from upstream = dL/dy (the residual's gradient
+ * is upstream itself): with z = x W^T + bias and dz = upstream act'(z), z
+ * computed again, grad_x = dz W, grad_weight = dz^T x, grad_bias = sum dz;
+ * each may be NULL.  The input is either x or, in 8 bits, codes and scales
+ * (gs3d_quantize_activations; x NULL then), which stand for x everywhere.
+ * Scratch: gs3d_linear_bwd_scratch_bytes. */
+typedef struct gs3d_linear_bwd_args {
+    int64_t rows;
+    int32_t inner, outer;
+    int32_t dtype, activation;
+    const void* x;
+    int64_t x_stride;
+    const int8_t* codes;
+    const uint8_t* scales;
+    const void* weight;
+    const void* bias;
+    const void* upstream;
+    int64_t upstream_stride;
+    void* grad_x;
+    void* grad_weight;
+    void* grad_bias;
+} gs3d_linear_bwd_args;
+
+size_t gs3d_linear_bwd_scratch_bytes(int64_t rows, int32_t inner, int32_t outer, int32_t dtype);
+int gs3d_linear_bwd(const gs3d_linear_bwd_args* args, void* scratch, size_t scratch_bytes, void* stream);
+
+/* y = act((x - mean) rstd weight + bias) over images of `pixels` rows each,
+ * mean and variance per image and group of channels / groups neighbouring
+ * channels, rstd = 1 / sqrt(variance + eps).  weight and bias may be NULL.
+ * statistics (images, groups, 2) receives mean and rstd for the backward
+ * pass.  Scratch: gs3d_group_norm_scratch_bytes, in both directions. */
+typedef struct gs3d_group_norm_args {
+    int32_t images;
+    int64_t pixels;
+    int32_t channels, groups;
+    int32_t dtype, activation;
+    float eps;
+    const void* x;
+    int64_t x_stride;
+    const void* weight;
+    const void* bias;
+    void* y;
+    float* statistics;
+} gs3d_group_norm_args;
+
+size_t gs3d_group_norm_scratch_bytes(int32_t images, int64_t pixels, int32_t channels, int32_t groups, int32_t dtype);
+int gs3d_group_norm_fwd(const gs3d_group_norm_args* args, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Gradients of gs3d_group_norm_fwd; x or codes and scales as in
+ * gs3d_linear_bwd (the statistics stay those of x).  Any gradient may be
+ * NULL. */
+typedef struct gs3d_group_norm_bwd_args {
+    int32_t images;
+    int64_t pixels;
+    int32_t channels, groups;
+    int32_t dtype, activation;
+    const void* x;
+    int64_t x_stride;
+    const int8_t* codes;
+    const uint8_t* scales;
+    const void* weight;
+    const void* bias;
+    const float* statistics;
+    const void* upstream;
+    int64_t upstream_stride;
+    void* grad_x;
+    void* grad_weight;
+    void* grad_bias;
+} gs3d_group_norm_bwd_args;
+
+int gs3d_group_norm_bwd(const gs3d_group_norm_bwd_args* args, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Activations in 8 bits: codes (rows, channels) int8 and scales (rows,
+ * ceil(channels / 32)) uint8.  A block of 32 neighbouring channels shares
+ * 2^e, the smallest with max |x| <= 127 2^e between e = -126 and 121
+ * (float16: 9), stored as e + 127; a code is x / 2^e rounded to the nearest
+ * integer, ties to even, at most 127 in size, and stands for code 2^e, which
+ * every type holds exactly.  A block that holds a value that is not finite
+ * has scale 255 and reads back as NaN.  out is contiguous. */
+int gs3d_quantize_activations(const void* x, int64_t x_stride, int64_t rows, int32_t channels, int32_t dtype,
+                              int8_t* codes, uint8_t* scales, void* stream);
+int gs3d_dequantize_activations(const int8_t* codes, const uint8_t* scales, int64_t rows, int32_t channels,
+                                int32_t dtype, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
