@@ -90,25 +90,52 @@ GS3D_DEV u32x4 pack(const float (&v)[8]) {
     return u32x4{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
 }
 
-// The VEC<T> elements of a row of `count` from element `at` on; those past
-// the row's end are zero and never read.
+// The VEC<T> elements of a row of `count` from element `at` on, in two steps
+// so that a load may be in flight while other work is done: issue_row starts
+// it, finish_row makes the elements past the row's end zero.  A vector that
+// would reach past the end is read from the row's last VEC<T> elements and
+// shifted down, so nothing beyond the row is read.  Rows shorter than a
+// vector are read element by element; a row of no channels is not read.
+template <int UNIT_BITS>
+GS3D_DEV u32x4 shift_down(u32x4 raw, int units) {
+    if (units * UNIT_BITS >= 128) return u32x4{0u, 0u, 0u, 0u};
+    uint64_t lo = (uint64_t)raw[1] << 32 | raw[0], hi = (uint64_t)raw[3] << 32 | raw[2];
+    int bits = units * UNIT_BITS;
+    if (bits >= 64) lo = hi, hi = 0u, bits -= 64;
+    lo = lo >> bits | (hi << 1) << (63 - bits);
+    hi >>= bits;
+    return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
 template <class T>
-GS3D_DEV u32x4 load_row(const T* row, int at, int count) {
-    if (at + VEC<T> <= count) return load16(row + at);
+GS3D_DEV u32x4 issue_row(const T* row, int at, int count) {
+    constexpr int E = VEC<T>;
+    if (count >= E) return load16(row + (at < count - E ? at : count - E));
     u32x4 raw = {0u, 0u, 0u, 0u};
-    if (at < count) {
+    if (count <= 0) return raw;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int k = at + i < count ? at + i : count - 1;
         if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (at + i < count) raw[i] = reinterpret_cast<const uint32_t*>(row)[at + i];
+            const uint32_t v = reinterpret_cast<const uint32_t*>(row)[k];
+            raw[i] = at + i < count ? v : 0u;
         } else {
-            const uint16_t* half = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (at + i < count) raw[i / 2] |= (uint32_t)half[at + i] << (16 * (i & 1));
+            const uint32_t v = reinterpret_cast<const uint16_t*>(row)[k];
+            raw[i / 2] |= at + i < count ? v << (16 * (i & 1)) : 0u;
         }
     }
     return raw;
+}
+template <class T>
+GS3D_DEV u32x4 finish_row(u32x4 raw, int at, int count) {
+    constexpr int E = VEC<T>;
+    const int over = at + E - count;
+    if (count >= E && over > 0) return shift_down<8 * (int)sizeof(T)>(raw, over);
+    return raw;
+}
+template <class T>
+GS3D_DEV u32x4 load_row(const T* row, int at, int count) {
+    return finish_row<T>(issue_row(row, at, count), at, count);
 }
 
 template <class T>
@@ -132,27 +159,89 @@ GS3D_DEV void store_row(T* row, int at, int count, u32x4 raw) {
 // ---------------------------------------------------------------------------
 // Activations (GS3D_ACT_*).  The kind is uniform over a launch.
 // ---------------------------------------------------------------------------
-GS3D_DEV float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+// exp2 on the hardware's 1-ulp instruction; results below 2^-126 are zero.
+GS3D_DEV float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+GS3D_DEV float rcp_fast(float v) { return __builtin_amdgcn_rcpf(v); }
 
-// Distribution function of the normal distribution.
-GS3D_DEV float normal_below(float z) { return 0.5f + 0.5f * erff(z * 0.70710678f); }
+GS3D_DEV float sigmoid(float z) { return rcp_fast(1.0f + exp2_fast(z * -1.44269504f)); }
 
-GS3D_DEV float activate(float z, int kind) {
-    if (kind == GS3D_ACT_SILU) return z * sigmoid(z);
-    if (kind == GS3D_ACT_GELU) return z * normal_below(z);
-    if (kind == GS3D_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays
+// The normal distribution's upper tail at |z|, and e^(-z^2/2) on the way:
+// Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (erfc by
+// a polynomial in 1 / (1 + p x) times e^(-x^2), x = |z| / sqrt 2, absolute
+// error 1.5e-7), with the half and the sqrt 2 folded into the constants.  17
+// issue slots (the exponential and the reciprocal are quarter rate), against
+// over 40 for the library's erf, which bounded the products' epilogues.
+GS3D_DEV float normal_tail(float z, float& bell) {
+    const float t = rcp_fast(__builtin_fmaf(__builtin_fabsf(z), 0.23164188f, 1.0f));
+    bell = exp2_fast(z * z * -0.72134752f);
+    float p = 0.53070271f;
+    p = __builtin_fmaf(p, t, -0.72657601f);
+    p = __builtin_fmaf(p, t, 0.71070687f);
+    p = __builtin_fmaf(p, t, -0.14224837f);
+    p = __builtin_fmaf(p, t, 0.12741480f);
+    return p * t * bell;
+}
+
+// z Phi(z) = max(z, 0) - |z| tail(|z|): no difference of near values.  The
+// tail is zero long before 64; past it an infinite z would meet a zero.
+GS3D_DEV float gelu(float z) {
+    float bell;
+    const float tail = normal_tail(z, bell);
+    return __builtin_fmaf(-__builtin_fminf(__builtin_fabsf(z), 64.0f), tail, z < 0.0f ? 0.0f : z);
+}
+
+template <int KIND>
+GS3D_DEV float activate_as(float z) {
+    if constexpr (KIND == GS3D_ACT_SILU) return z * sigmoid(z);
+    if constexpr (KIND == GS3D_ACT_GELU) return gelu(z);
+    if constexpr (KIND == GS3D_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays
     return z;
 }
 
-// Derivative of activate at z.
-GS3D_DEV float slope(float z, int kind) {
-    if (kind == GS3D_ACT_SILU) {
+// Derivative of activate_as at z.
+template <int KIND>
+GS3D_DEV float slope_as(float z) {
+    if constexpr (KIND == GS3D_ACT_SILU) {
         const float s = sigmoid(z);
         return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
     }
-    if (kind == GS3D_ACT_GELU) return __builtin_fmaf(z * 0.39894228f, __expf(-0.5f * z * z), normal_below(z));
-    if (kind == GS3D_ACT_RELU) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
+    if constexpr (KIND == GS3D_ACT_GELU) {
+        float bell;
+        const float tail = normal_tail(z, bell);
+        return __builtin_fmaf(__builtin_amdgcn_fmed3f(z, -64.0f, 64.0f) * 0.39894228f, bell,
+                              z < 0.0f ? tail : 1.0f - tail);
+    }
+    if constexpr (KIND == GS3D_ACT_RELU) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
     return 1.0f;
+}
+
+// A vector at a time, the (uniform) kind looked at once.
+template <int E>
+GS3D_DEV void activate(float (&z)[E], int kind) {
+    if (kind == GS3D_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) z[i] = activate_as<GS3D_ACT_SILU>(z[i]);
+    } else if (kind == GS3D_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) z[i] = activate_as<GS3D_ACT_GELU>(z[i]);
+    } else if (kind == GS3D_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) z[i] = activate_as<GS3D_ACT_RELU>(z[i]);
+    }
+}
+// g[i] *= slope at z[i].
+template <int E>
+GS3D_DEV void pull_back(float (&g)[E], const float (&z)[E], int kind) {
+    if (kind == GS3D_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) g[i] *= slope_as<GS3D_ACT_SILU>(z[i]);
+    } else if (kind == GS3D_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) g[i] *= slope_as<GS3D_ACT_GELU>(z[i]);
+    } else if (kind == GS3D_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) g[i] *= slope_as<GS3D_ACT_RELU>(z[i]);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -195,40 +284,82 @@ struct Q8Rows {
 };
 
 // The VEC<T> values of one row from channel `at` on (a multiple of VEC<T>),
-// zero past the row's end.
+// zero past the row's end, in the same two steps.
+struct Q8Raw {
+    uint64_t codes;
+    uint32_t scale;
+};
+
 template <class T>
-GS3D_DEV u32x4 load_row_q8(const Q8Rows& q, int64_t row, int at) {
+GS3D_DEV Q8Raw issue_row_q8(const Q8Rows& q, int64_t row, int at) {
     constexpr int E = VEC<T>;
-    float v[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = 0.0f;
-    if (at < q.channels) {
-        const int8_t* p = q.codes + row * q.channels + at;
-        const float scale = q8_scale(q.scales[row * ((q.channels + 31) >> 5) + (at >> 5)]);
-        uint32_t word[E / 4];
-        if (at + E <= q.channels) {
-            if constexpr (E == 8) {
-                const u32x2 w = *reinterpret_cast<const u32x2_at1*>(p);
-                word[0] = w[0];
-                word[1] = w[1];
-            } else {
-                word[0] = *reinterpret_cast<const u32_at1*>(p);
-            }
+    const int8_t* p = q.codes + row * q.channels;
+    Q8Raw raw = {0u, 0u};
+    if (q.channels <= 0) return raw;
+    const int block = (at < q.channels ? at : q.channels - 1) >> 5;
+    raw.scale = q.scales[row * ((q.channels + 31) >> 5) + block];
+    if (q.channels >= E) {
+        p += at < q.channels - E ? at : q.channels - E;
+        if constexpr (E == 8) {
+            const u32x2 w = *reinterpret_cast<const u32x2_at1*>(p);
+            raw.codes = (uint64_t)w[1] << 32 | w[0];
         } else {
-#pragma unroll
-            for (int i = 0; i < E / 4; ++i) word[i] = 0u;
-#pragma unroll
-            for (int i = 0; i < E; ++i)
-                if (at + i < q.channels) word[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+            raw.codes = *reinterpret_cast<const u32_at1*>(p);
         }
+    } else {
+        raw.codes = 0u;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const float value = (float)(int)(int8_t)(word[i / 4] >> (8 * (i & 3))) * scale;
-            v[i] = at + i < q.channels ? value : 0.0f;  // a NaN block ends with its row
+            const uint32_t v = (uint8_t)p[at + i < q.channels ? at + i : q.channels - 1];
+            raw.codes |= (uint64_t)(at + i < q.channels ? v : 0u) << (8 * i);
         }
+    }
+    return raw;
+}
+
+// An element past the row's end is zero also where the row ends in a block
+// that reads back as NaN.
+template <class T>
+GS3D_DEV u32x4 finish_row_q8(Q8Raw raw, int at, int channels) {
+    constexpr int E = VEC<T>;
+    const int over = at + E - channels;
+    if (channels >= E && over > 0) raw.codes = over >= E ? 0u : raw.codes >> (8 * over);
+    const float scale = q8_scale(raw.scale);
+    float v[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = (float)(int)(int8_t)(raw.codes >> (8 * i)) * scale;
+    if (over > 0) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = at + i < channels ? v[i] : 0.0f;
     }
     return pack<T>(v);
 }
+template <class T>
+GS3D_DEV u32x4 load_row_q8(const Q8Rows& q, int64_t row, int at) {
+    return finish_row_q8<T>(issue_row_q8<T>(q, row, at), at, q.channels);
+}
+
+// Rows of activations, plain or in 8 bits, behind one pair of steps.
+struct Rows {
+    const void* x;
+    int64_t ldx;
+    Q8Rows q8;
+    int channels;
+};
+template <class T, bool Q8>
+struct RowRaw {
+    u32x4 raw;
+    GS3D_DEV void issue(const Rows& a, int64_t row, int at) {
+        raw = issue_row(static_cast<const T*>(a.x) + row * a.ldx, at, a.channels);
+    }
+    GS3D_DEV u32x4 finish(const Rows& a, int at) const { return finish_row<T>(raw, at, a.channels); }
+};
+template <class T>
+struct RowRaw<T, true> {
+    Q8Raw raw;
+    GS3D_DEV void issue(const Rows& a, int64_t row, int at) { raw = issue_row_q8<T>(a.q8, row, at); }
+    GS3D_DEV u32x4 finish(const Rows& a, int at) const { return finish_row_q8<T>(raw, at, a.channels); }
+};
 
 // ---------------------------------------------------------------------------
 // Matrix fragments.  A fragment is 16 bytes a lane: lane l holds row l % 16
@@ -255,6 +386,43 @@ GS3D_DEV f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
         for (int i = 0; i < 4; ++i)
             c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
         return c;
+    }
+}
+
+// Column of row r of tile t in an operand whose rows become an output's
+// columns.  A lane ends up with rows 4q..4q+3 of every tile; for 16-bit types
+// two tiles are dealt out so that their eight values are neighbours, 16 bytes
+// of an output row.
+template <class T>
+GS3D_DEV int tile_column(int t, int r) {
+    if constexpr (sizeof(T) == 4) return 16 * t + r;
+    return 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3);
+}
+
+// Fragment of the transpose of a row-major LDS tile (`pitch` 16-byte units a
+// row): lane l gets one column of 16 and the VEC<T> rows from
+// row0 + VEC<T> (l / 16) on.  DEALT columns are tile_column's, else 16 t + r.
+// 16-bit types use the transposing LDS read, of which 16 lanes fetch four rows
+// of 16 columns (lane s the four columns 4 (s % 4).. of row s / 4, from any
+// address) and lane i receives column i of the four rows; float reads words.
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+template <class T, bool DEALT>
+GS3D_DEV u32x4 read_transposed(const u32x4* tile, int pitch, int row0, int t, int lane) {
+    const int s = lane & 15, q = lane >> 4;
+    if constexpr (sizeof(T) == 4) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(tile) + (row0 + 4 * q) * pitch * 4 + 16 * t + s;
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = p[i * pitch * 4];
+        return v;
+    } else {
+        const int column = DEALT ? 32 * (t >> 1) + 4 * (t & 1) + 8 * (s & 3) : 16 * t + 4 * (s & 3);
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(tile) + (row0 + 8 * q + (s >> 2)) * pitch * 8 + column;
+        typedef __attribute__((address_space(3))) i16x4* lds_ptr;
+        const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+        const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * pitch * 8));
+        const u32x2 lo = __builtin_bit_cast(u32x2, a), hi = __builtin_bit_cast(u32x2, b);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
 }
 

@@ -29,12 +29,6 @@ struct NormShape {
     float eps;
 };
 
-struct NormRows {
-    const void* x;
-    int64_t ldx;
-    Q8Rows q8;
-};
-
 struct NormParams {
     const void* gamma;  // channels, or NULL: 1
     const void* beta;   // channels, or NULL: 0
@@ -57,12 +51,6 @@ GS3D_DEV NormThread norm_thread(int channels) {
     t.at = (first + threadIdx.x % t.width) * E;
     t.live = t.slot < t.slots;
     return t;
-}
-
-template <class T, bool Q8>
-GS3D_DEV u32x4 norm_load(const NormRows& a, int64_t row, int at, int channels) {
-    if constexpr (Q8) return load_row_q8<T>(a.q8, row, at);
-    else return load_row(static_cast<const T*>(a.x) + row * a.ldx, at, channels);
 }
 
 // Per-channel constants of a thread: u = (x - mean) scale + beta.
@@ -91,7 +79,7 @@ GS3D_DEV void merge_moments(float& n, float& mean, float& m2, float nb, float mb
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void norm_statistics_kernel(NormShape s, NormRows a, float2* __restrict__ part) {
+__global__ __launch_bounds__(256) void norm_statistics_kernel(NormShape s, Rows a, float2* __restrict__ part) {
     constexpr int E = VEC<T>;
     constexpr int U = 4;  // pixels whose loads are in flight together
     const NormThread t = norm_thread<E>(s.channels);
@@ -102,17 +90,17 @@ __global__ __launch_bounds__(256) void norm_statistics_kernel(NormShape s, NormR
     for (int i = 0; i < E; ++i) mean[i] = m2[i] = 0.0f;
     if (t.live) {
         for (int64_t p = begin + t.slot; p < end; p += U * t.slots) {
-            u32x4 raw[U];
+            RowRaw<T, false> raw[U];
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 const int64_t row = p + k * t.slots;
-                raw[k] = norm_load<T, false>(a, base + (row < end ? row : p), t.at, s.channels);
+                raw[k].issue(a, base + (row < end ? row : p), t.at);
             }
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 if (p + k * t.slots >= end) break;
                 float v[E];
-                unpack<T>(raw[k], v);
+                unpack<T>(raw[k].finish(a, t.at), v);
                 n += 1.0f;
                 const float share = __builtin_amdgcn_rcpf(n);
 #pragma unroll
@@ -124,22 +112,37 @@ __global__ __launch_bounds__(256) void norm_statistics_kernel(NormShape s, NormR
             }
         }
     }
-    __shared__ float lds[3][256];
+    // The block's pixels of a channel together, halving the slots.
+    __shared__ float lds[2 * E + 1][256];
+    for (int live = t.slots; live > 1; live = (live + 1) / 2) {
+        const int half = (live + 1) / 2;
+        __syncthreads();
+        if (t.slot >= half && t.slot < live) {
+            lds[2 * E][threadIdx.x] = n;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        __syncthreads();
-        lds[0][threadIdx.x] = n;
-        lds[1][threadIdx.x] = mean[i];
-        lds[2][threadIdx.x] = m2[i];
-        __syncthreads();
-        if (t.slot == 0 && t.at + i < s.channels) {
-            float tn = n, tm = mean[i], t2 = m2[i];
-            for (int k = 1; k < t.slots; ++k) {
-                const int j = threadIdx.x + k * t.width;
-                merge_moments(tn, tm, t2, lds[0][j], lds[1][j], lds[2][j]);
-            }
-            part[((int64_t)blockIdx.y * s.strips + blockIdx.x) * s.channels + t.at + i] = float2{tm, t2};
+            for (int i = 0; i < E; ++i) lds[i][threadIdx.x] = mean[i], lds[E + i][threadIdx.x] = m2[i];
         }
+        __syncthreads();
+        if (t.slot + half < live) {
+            const int j = threadIdx.x + half * t.width;
+            const float nb = lds[2 * E][j], total = n + nb;
+            if (nb > 0.0f) {
+                const float share = nb / total, weight = n * share;
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const float d = lds[i][j] - mean[i];
+                    mean[i] = __builtin_fmaf(d, share, mean[i]);
+                    m2[i] += __builtin_fmaf(d * d, weight, lds[E + i][j]);
+                }
+                n = total;
+            }
+        }
+    }
+    if (t.slot == 0) {
+        float2* out = part + ((int64_t)blockIdx.y * s.strips + blockIdx.x) * s.channels + t.at;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (t.at + i < s.channels) out[i] = float2{mean[i], m2[i]};
     }
 }
 
@@ -178,7 +181,7 @@ __global__ __launch_bounds__(1024) void norm_merge_kernel(NormShape s, const flo
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, NormRows a, NormParams p, T* __restrict__ y) {
+__global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, Rows a, NormParams p, T* __restrict__ y) {
     constexpr int E = VEC<T>;
     constexpr int U = 4;
     const NormThread t = norm_thread<E>(s.channels);
@@ -188,27 +191,28 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, NormRows a
     float mean[E], rstd[E], scale[E], beta[E];
     norm_constants<T, E>(s, p, blockIdx.y, t.at, mean, rstd, scale, beta);
     for (int64_t row = begin + t.slot; row < end; row += U * t.slots) {
-        u32x4 raw[U];
+        RowRaw<T, false> raw[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int64_t at = row + k * t.slots;
-            raw[k] = norm_load<T, false>(a, base + (at < end ? at : row), t.at, s.channels);
+            raw[k].issue(a, base + (at < end ? at : row), t.at);
         }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int64_t at = row + k * t.slots;
             if (at >= end) break;
             float v[E];
-            unpack<T>(raw[k], v);
+            unpack<T>(raw[k].finish(a, t.at), v);
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = activate(__builtin_fmaf(v[i] - mean[i], scale[i], beta[i]), s.act);
+            for (int i = 0; i < E; ++i) v[i] = __builtin_fmaf(v[i] - mean[i], scale[i], beta[i]);
+            activate(v, s.act);
             store_row(y + (base + at) * s.channels, t.at, s.channels, pack<T>(v));
         }
     }
 }
 
 template <class T, bool Q8>
-__global__ __launch_bounds__(256) void norm_sums_kernel(NormShape s, NormRows a, NormParams p, const T* __restrict__ dy,
+__global__ __launch_bounds__(256) void norm_sums_kernel(NormShape s, Rows a, NormParams p, const T* __restrict__ dy,
                                                         int64_t ldy, float2* __restrict__ part) {
     constexpr int E = VEC<T>;
     constexpr int U = 2;
@@ -222,44 +226,54 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(NormShape s, NormRows a,
         float mean[E], scale[E], beta[E];
         norm_constants<T, E>(s, p, blockIdx.y, t.at, mean, rstd, scale, beta);
         for (int64_t row = begin + t.slot; row < end; row += U * t.slots) {
-            u32x4 raw[U], up[U];
+            RowRaw<T, Q8> raw[U];
+            u32x4 up[U];
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 const int64_t r = row + k * t.slots, at = base + (r < end ? r : row);
-                raw[k] = norm_load<T, Q8>(a, at, t.at, s.channels);
-                up[k] = load_row(dy + at * ldy, t.at, s.channels);
+                raw[k].issue(a, at, t.at);
+                up[k] = issue_row(dy + at * ldy, t.at, s.channels);
             }
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 if (row + k * t.slots >= end) break;
-                float v[E], g[E];
-                unpack<T>(raw[k], v);
-                unpack<T>(up[k], g);
+                float v[E], u[E], g[E];
+                unpack<T>(raw[k].finish(a, t.at), v);
+                unpack<T>(finish_row<T>(up[k], t.at, s.channels), g);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const float d = v[i] - mean[i];
-                    const float dz = g[i] * slope(__builtin_fmaf(d, scale[i], beta[i]), s.act);
-                    s1[i] += dz;
-                    s2[i] = __builtin_fmaf(dz, d, s2[i]);
+                    v[i] -= mean[i];
+                    u[i] = __builtin_fmaf(v[i], scale[i], beta[i]);
+                }
+                pull_back(g, u, s.act);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    s1[i] += g[i];
+                    s2[i] = __builtin_fmaf(g[i], v[i], s2[i]);
                 }
             }
         }
     }
-    __shared__ float lds[2][256];
+    __shared__ float lds[2 * E][256];
+    for (int live = t.slots; live > 1; live = (live + 1) / 2) {
+        const int half = (live + 1) / 2;
+        __syncthreads();
+        if (t.slot >= half && t.slot < live) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        __syncthreads();
-        lds[0][threadIdx.x] = s1[i];
-        lds[1][threadIdx.x] = s2[i];
-        __syncthreads();
-        if (t.slot == 0 && t.at + i < s.channels) {
-            float a1 = s1[i], a2 = s2[i];
-            for (int k = 1; k < t.slots; ++k) {
-                a1 += lds[0][threadIdx.x + k * t.width];
-                a2 += lds[1][threadIdx.x + k * t.width];
-            }
-            part[((int64_t)blockIdx.y * s.strips + blockIdx.x) * s.channels + t.at + i] = float2{a1, a2 * rstd[i]};
+            for (int i = 0; i < E; ++i) lds[i][threadIdx.x] = s1[i], lds[E + i][threadIdx.x] = s2[i];
         }
+        __syncthreads();
+        if (t.slot + half < live) {
+            const int j = threadIdx.x + half * t.width;
+#pragma unroll
+            for (int i = 0; i < E; ++i) s1[i] += lds[i][j], s2[i] += lds[E + i][j];
+        }
+    }
+    if (t.slot == 0) {
+        float2* out = part + ((int64_t)blockIdx.y * s.strips + blockIdx.x) * s.channels + t.at;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (t.at + i < s.channels) out[i] = float2{s1[i], s2[i] * rstd[i]};
     }
 }
 
@@ -331,7 +345,7 @@ __global__ __launch_bounds__(256) void norm_params_kernel(int images, int channe
 }
 
 template <class T, bool Q8>
-__global__ __launch_bounds__(256) void norm_grad_kernel(NormShape s, NormRows a, NormParams p, const T* __restrict__ dy,
+__global__ __launch_bounds__(256) void norm_grad_kernel(NormShape s, Rows a, NormParams p, const T* __restrict__ dy,
                                                         int64_t ldy, const float2* __restrict__ pulls,
                                                         T* __restrict__ dx) {
     constexpr int E = VEC<T>;
@@ -353,26 +367,30 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormShape s, NormRows a,
         along[i] = rstd * rstd * pull.y;
     }
     for (int64_t row = begin + t.slot; row < end; row += U * t.slots) {
-        u32x4 raw[U], up[U];
+        RowRaw<T, Q8> raw[U];
+        u32x4 up[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int64_t r = row + k * t.slots, at = base + (r < end ? r : row);
-            raw[k] = norm_load<T, Q8>(a, at, t.at, s.channels);
-            up[k] = load_row(dy + at * ldy, t.at, s.channels);
+            raw[k].issue(a, at, t.at);
+            up[k] = issue_row(dy + at * ldy, t.at, s.channels);
         }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int64_t at = row + k * t.slots;
             if (at >= end) break;
-            float v[E], g[E];
-            unpack<T>(raw[k], v);
-            unpack<T>(up[k], g);
+            float v[E], u[E], g[E];
+            unpack<T>(raw[k].finish(a, t.at), v);
+            unpack<T>(finish_row<T>(up[k], t.at, s.channels), g);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float d = v[i] - mean[i];
-                const float dz = g[i] * slope(__builtin_fmaf(d, scale[i], beta[i]), s.act);
-                v[i] = __builtin_fmaf(-d, along[i], __builtin_fmaf(scale[i], dz, -level[i]));
+                v[i] -= mean[i];
+                u[i] = __builtin_fmaf(v[i], scale[i], beta[i]);
             }
+            pull_back(g, u, s.act);
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                v[i] = __builtin_fmaf(-v[i], along[i], __builtin_fmaf(scale[i], g[i], -level[i]));
             store_row(dx + (base + at) * s.channels, t.at, s.channels, pack<T>(v));
         }
     }
@@ -414,7 +432,7 @@ template <class T>
 static int norm_fwd(const gs3d_group_norm_args& g, void* scratch, hipStream_t stream) {
     NormShape s = norm_shape(g.images, g.pixels, g.channels, g.groups, g.dtype);
     s.act = g.activation, s.eps = g.eps;
-    const NormRows a{g.x, g.x_stride, {}};
+    const Rows a{g.x, g.x_stride, {}, g.channels};
     float2* part = static_cast<float2*>(scratch);
     float2* stats = reinterpret_cast<float2*>(g.statistics);
     const dim3 grid = norm_grid(s, g.dtype);
@@ -429,7 +447,7 @@ template <class T, bool Q8>
 static int norm_bwd(const gs3d_group_norm_bwd_args& g, char* scratch, hipStream_t stream) {
     NormShape s = norm_shape(g.images, g.pixels, g.channels, g.groups, g.dtype);
     s.act = g.activation;
-    const NormRows a{g.x, g.x_stride, {g.codes, g.scales, g.channels}};
+    const Rows a{g.x, g.x_stride, {g.codes, g.scales, g.channels}, g.channels};
     const NormParams p{g.weight, g.bias, reinterpret_cast<const float2*>(g.statistics)};
     float2* part = reinterpret_cast<float2*>(scratch);
     float2* sums = reinterpret_cast<float2*>(scratch + norm_part_bytes(s));

@@ -1,0 +1,597 @@
+// Per-pixel products of the feature decoder: y = act(x W^T + b) + r and its
+// gradients, over rows x (pixels) that are many and channels that are few.
+// Included by linear_f32.hip, linear_bf16.hip and linear_f16.hip.
+//
+//   linear_stream_kernel     rows times weights that lie in LDS whole, while the
+//                            rows stream past: every product whose contracted
+//                            dimension has at most 8 chunks
+//   linear_rows_kernel       the same for longer ones, the weights in steps
+//   linear_bwd_fused_kernel  the whole backward pass in one (linear_fused.hpp),
+//                            where its weights and their gradient fit a block
+//   linear_gradw_kernel      otherwise: dW = dz^T x and db = sum dz, split over
+//                            the rows, after dz and dx from the kernels above
+//   sum_splits_kernel        the blocks' partial sums in a fixed order
+//
+// The products of the forward (EPI 0) end in act and r; those of the backward
+// (EPI 1) in dz = dy act'(x W^T + b), z computed again rather than kept.
+// Products of 16-bit types go through matrix instructions with sums in 32
+// bits.  dz is rounded to the element type once, as the operand of the two
+// products that follow it.
+#pragma once
+
+#include "linear_fused.hpp"
+
+namespace gs3d {
+
+struct LinearRows {
+    Rows x;              // rows x K
+    const void* w;       // N x K
+    const void* bias;    // N or NULL
+    const void* other;   // EPI 0: residual or NULL; EPI 1: dy
+    int64_t ldo;
+    void* y;             // rows x N
+    int64_t rows;
+    int K, N, act, n_tiles, strips;
+};
+
+// Blocks b, b + 8, b + 16, ... run on one XCD: the column tiles of a range of
+// rows are dealt to one of them, whose L2 then holds x once.
+GS3D_DEV void xcd_block(const LinearRows& a, int64_t& row_block, int& n_tile) {
+    const int64_t local = blockIdx.x >> 3;
+    row_block = (local / a.n_tiles) * 8 + (blockIdx.x & 7);
+    n_tile = (int)(local % a.n_tiles);
+}
+
+// The end of a product for one lane's vector of E neighbouring outputs.
+template <class T, int EPI, int E>
+GS3D_DEV u32x4 linear_end(const LinearRows& a, float (&z)[E], u32x4 raw_other) {
+    float o[E];
+    if constexpr (EPI == 1) {
+        unpack<T>(raw_other, o);
+        pull_back(o, z, a.act);
+        return pack<T>(o);
+    } else {
+        activate(z, a.act);
+        if (a.other) {
+            unpack<T>(raw_other, o);
+#pragma unroll
+            for (int i = 0; i < E; ++i) z[i] += o[i];
+        }
+        return pack<T>(z);
+    }
+}
+
+// Wavefronts a SIMD that the stream kernel's registers leave room for.
+template <class T, bool Q8, int KCH, int NT>
+constexpr int stream_waves() {
+    if (sizeof(T) == 4) return KCH == 8 ? (NT == 8 ? 1 : 2) : KCH == 4 ? (NT == 8 ? 2 : 3) : NT == 8 ? 3 : 4;
+    if (Q8) return KCH == 8 ? 1 : KCH == 4 ? (NT == 8 ? 2 : 3) : 4;
+    return KCH == 8 ? 2 : NT == 8 ? 4 : 5 - (KCH == 4 ? 1 : 0);
+}
+
+// A block of 4 wavefronts holds the weights of 16 NT columns in LDS, in
+// fragment order (one 1 KB run per chunk and tile, read without conflicts),
+// and takes strips of 16 rows from a range of a.strips of them.  A wavefront
+// reads its strip straight into fragments, 64 bytes of a row at a time, the
+// next strip while this one is multiplied; the wavefronts never wait for one
+// another.  W's rows are the first operand, so a lane ends with 16 bytes of
+// one output row.  HBM bounds it while K and N are small.
+template <class T, bool Q8, int EPI, int KCH, int NT>
+__global__ __launch_bounds__(256, (stream_waves<T, Q8, KCH, NT>())) void linear_stream_kernel(LinearRows a) {
+    constexpr int E = VEC<T>;
+    constexpr int KC = CHUNK<T>;
+    constexpr int TG = KC / 16;  // tiles of a lane's 16-byte output vector
+    constexpr int G = NT / TG;
+    __shared__ u32x4 w_lds[KCH * NT * 64];
+    __shared__ float bias_lds[16 * NT];
+
+    int64_t row_block;
+    int n_tile;
+    xcd_block(a, row_block, n_tile);
+    const int n0 = n_tile * 16 * NT;
+    const int64_t first = row_block * a.strips * 16;
+    if (first >= a.rows) return;
+    const int64_t end = first + a.strips * 16 < a.rows ? first + a.strips * 16 : a.rows;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 15, q = lane >> 4;
+    const T* w = static_cast<const T*>(a.w);
+    const T* other = static_cast<const T*>(a.other);
+    T* y = static_cast<T*>(a.y);
+
+#pragma unroll
+    for (int i = 0; i < (KCH * NT + 3) / 4; ++i) {
+        const int slot = i * 256 + tid;
+        if (KCH * NT % 4 != 0 && slot >= KCH * NT * 64) break;
+        const int c = slot / (NT * 64), t = (slot / 64) % NT, l = slot & 63;
+        const int n = n0 + tile_column<T>(t, l & 15), k = c * KC + (l >> 4) * E;
+        w_lds[slot] = n < a.N ? load_row(w + (int64_t)n * a.K, k, a.K) : u32x4{0u, 0u, 0u, 0u};
+    }
+    if (tid < 16 * NT)
+        bias_lds[tid] = a.bias && n0 + tid < a.N ? to_f32(static_cast<const T*>(a.bias)[n0 + tid]) : 0.0f;
+    __syncthreads();
+
+    RowRaw<T, Q8> xr[KCH];
+    auto load = [&](int64_t m) {
+        m = m < end ? m : end - 1;  // rows past the end repeat the last one and are not stored
+#pragma unroll
+        for (int c = 0; c < KCH; ++c) xr[c].issue(a.x, m, c * KC + q * E);
+    };
+    int64_t m = first + wave * 16 + r;
+    load(m);
+    for (; m - r < end; m += 64) {
+        u32x4 xf[KCH], o[G];
+#pragma unroll
+        for (int c = 0; c < KCH; ++c) xf[c] = xr[c].finish(a.x, c * KC + q * E);
+        if (EPI == 1 || other) {
+            const int64_t at = m < end ? m : end - 1;
+#pragma unroll
+            for (int g = 0; g < G; ++g) o[g] = issue_row(other + at * a.ldo, n0 + g * KC + q * E, a.N);
+        }
+        if (m - r + 64 < end) load(m + 64);
+        // The weights stay in LDS: hoisted out of the loop they would take
+        // every register (128 at 4 chunks x 8 tiles).
+        int mine = lane;
+        asm volatile("" : "+v"(mine));
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            f32x4 acc[TG];
+#pragma unroll
+            for (int t = 0; t < TG; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < KCH; ++c)
+#pragma unroll
+                for (int t = 0; t < TG; ++t)
+                    acc[t] = multiply<T>(w_lds[(c * NT + g * TG + t) * 64 + mine], xf[c], acc[t]);
+            const int at = g * KC + q * E;
+            float z[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) z[i] = acc[i / 4][i & 3] + bias_lds[at + i];
+            u32x4 raw = {0u, 0u, 0u, 0u};
+            if (EPI == 1 || other) raw = finish_row<T>(o[g], n0 + at, a.N);
+            raw = linear_end<T, EPI, E>(a, z, raw);
+            if (m < end) store_row(y + m * a.N, n0 + at, a.N, raw);
+        }
+    }
+}
+
+// Longer contracted dimensions: a block of 4 wavefronts computes 64 RS rows x
+// 16 NT columns, the weights' fragments of CH chunks at a time through LDS for
+// all four, the next step's operands loaded while this one's are multiplied.
+template <class T, bool Q8, int EPI, int RS, int NT>
+__global__ __launch_bounds__(256) void linear_rows_kernel(LinearRows a) {
+    constexpr int E = VEC<T>;
+    constexpr int KC = CHUNK<T>;
+    constexpr int CH = 2;            // chunks of the contracted dimension a step
+    constexpr int WL = CH * NT / 4;  // fragments of W a thread brings in
+    constexpr int TG = KC / 16;
+    __shared__ u32x4 w_lds[CH * NT * 64];
+    __shared__ float bias_lds[16 * NT];
+
+    int64_t row_block;
+    int n_tile;
+    xcd_block(a, row_block, n_tile);
+    const int n0 = n_tile * 16 * NT;
+    const int64_t first = row_block * (64 * RS);
+    if (first >= a.rows) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 15, q = lane >> 4;
+    const T* w = static_cast<const T*>(a.w);
+
+    int64_t row[RS];
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+        const int64_t m = first + wave * (16 * RS) + 16 * s + r;
+        row[s] = m < a.rows ? m : a.rows - 1;  // rows past the end repeat the last one and are not stored
+    }
+    if (tid < 16 * NT) {
+        const int n = n0 + tid;
+        bias_lds[tid] = a.bias && n < a.N ? to_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
+    }
+
+    u32x4 wr[WL];
+    RowRaw<T, Q8> xr[RS][CH];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+            const int slot = i * 256 + tid;
+            const int c = slot / (NT * 64), t = (slot / 64) % NT, l = slot & 63;
+            const int n = n0 + tile_column<T>(t, l & 15);
+            wr[i] = issue_row(w + (int64_t)(n < a.N ? n : a.N - 1) * a.K, k0 + c * KC + (l >> 4) * E, a.K);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int s = 0; s < RS; ++s) xr[s][c].issue(a.x, row[s], k0 + c * KC + q * E);
+    };
+
+    f32x4 acc[RS][NT];
+#pragma unroll
+    for (int s = 0; s < RS; ++s)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[s][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    load(0);
+    for (int k0 = 0; k0 < a.K; k0 += CH * KC) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+            const int slot = i * 256 + tid;
+            const int c = slot / (NT * 64), t = (slot / 64) % NT, l = slot & 63;
+            const u32x4 v = finish_row<T>(wr[i], k0 + c * KC + (l >> 4) * E, a.K);
+            w_lds[slot] = n0 + tile_column<T>(t, l & 15) < a.N ? v : u32x4{0u, 0u, 0u, 0u};
+        }
+        u32x4 xc[RS][CH];
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) xc[s][c] = xr[s][c].finish(a.x, k0 + c * KC + q * E);
+        __syncthreads();
+        if (k0 + CH * KC < a.K) load(k0 + CH * KC);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const u32x4 wf = w_lds[(c * NT + t) * 64 + lane];
+#pragma unroll
+                for (int s = 0; s < RS; ++s) acc[s][t] = multiply<T>(wf, xc[s][c], acc[s][t]);
+            }
+    }
+
+    T* y = static_cast<T*>(a.y);
+    const T* other = static_cast<const T*>(a.other);
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+        const int64_t m = first + wave * (16 * RS) + 16 * s + r;
+        if (m >= a.rows) continue;
+#pragma unroll
+        for (int g = 0; g < NT / TG; ++g) {
+            const int at = g * KC + q * E;  // column within the block's tile
+            if (n0 + at >= a.N) continue;
+            float z[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) z[i] = acc[s][g * TG + i / 4][i & 3] + bias_lds[at + i];
+            u32x4 raw = {0u, 0u, 0u, 0u};
+            if (EPI == 1 || other) raw = load_row(other + m * a.ldo, n0 + at, a.N);
+            store_row(y + m * a.N, n0 + at, a.N, linear_end<T, EPI, E>(a, z, raw));
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ w, int n, int k, T* __restrict__ out) {
+    __shared__ T tile[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    for (int i = ty; i < 32; i += 8) {
+        const int row = blockIdx.y * 32 + i, col = blockIdx.x * 32 + tx;
+        if (row < n && col < k) tile[i][tx] = w[(int64_t)row * k + col];
+    }
+    __syncthreads();
+    for (int i = ty; i < 32; i += 8) {
+        const int row = blockIdx.x * 32 + i, col = blockIdx.y * 32 + tx;
+        if (row < k && col < n) out[(int64_t)row * n + col] = tile[tx][i];
+    }
+}
+
+struct LinearGradW {
+    Rows x;          // channels 0: only db
+    const void* dz;
+    int64_t ldz;
+    int64_t rows, rows_per_split;
+    int N, n_tiles, k_tiles;
+    float* part;     // splits x (N K + N)
+    int K;
+};
+
+// dW tile of 32 A columns of dz x 32 B columns of x over one split's rows.
+// The contracted dimension is the row, the slow one of both operands: they go
+// to LDS as they are, row by row, and are read transposed.  2 x 2 wavefronts
+// multiply 16 A x 16 B columns each.
+template <class T, bool Q8, int A, int B>
+__global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
+    constexpr int E = VEC<T>;
+    constexpr int KC = CHUNK<T>;
+    constexpr int MR = 2 * KC;                       // rows a step
+    constexpr int CZ = 32 * A / E, CX = 32 * B / E;  // vectors across dz's and x's tile
+    constexpr int PZ = CZ + 1, PX = CX + 1;          // pitches: the odd unit spreads rows over the banks
+    constexpr int LZ = (MR * CZ + 255) / 256, LX = (MR * CX + 255) / 256;
+    __shared__ u32x4 z_lds[MR * PZ];
+    __shared__ u32x4 x_lds[MR * PX];
+
+    int64_t b = blockIdx.x;
+    const int kt = (int)(b % a.k_tiles);
+    b /= a.k_tiles;
+    const int nt = (int)(b % a.n_tiles);
+    const int split = (int)(b / a.n_tiles);
+    const int n0 = nt * 32 * A, k0 = kt * 32 * B;
+    const int64_t begin = split * a.rows_per_split;
+    const int64_t end = begin + a.rows_per_split < a.rows ? begin + a.rows_per_split : a.rows;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 15, q = lane >> 4;
+    const int wn = wave >> 1, wk = wave & 1;
+    const bool sum_bias = kt == 0 && wk == 0;
+    const T* dz = static_cast<const T*>(a.dz);
+
+    u32x4 zr[LZ];
+    RowRaw<T, Q8> xr[LX];
+    auto load = [&](int64_t m0) {
+#pragma unroll
+        for (int i = 0; i < LZ; ++i) {
+            const int u = i * 256 + tid;
+            const int64_t m = m0 + u / CZ < end ? m0 + u / CZ : end - 1;
+            zr[i] = issue_row(dz + m * a.ldz, n0 + u % CZ * E, a.N);
+        }
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            const int u = i * 256 + tid;
+            const int64_t m = m0 + u / CX < end ? m0 + u / CX : end - 1;
+            xr[i].issue(a.x, m, k0 + u % CX * E);
+        }
+    };
+    auto store = [&](int64_t m0) {
+#pragma unroll
+        for (int i = 0; i < LZ; ++i) {
+            const int u = i * 256 + tid;
+            const u32x4 v = finish_row<T>(zr[i], n0 + u % CZ * E, a.N);
+            if (MR * CZ % 256 == 0 || u < MR * CZ)
+                z_lds[u / CZ * PZ + u % CZ] = m0 + u / CZ < end ? v : u32x4{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            const int u = i * 256 + tid;
+            const u32x4 v = xr[i].finish(a.x, k0 + u % CX * E);
+            if (MR * CX % 256 == 0 || u < MR * CX)
+                x_lds[u / CX * PX + u % CX] = m0 + u / CX < end ? v : u32x4{0u, 0u, 0u, 0u};
+        }
+    };
+
+    f32x4 acc[A][B], acc_b[A];
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+        acc_b[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < B; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float one[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) one[i] = 1.0f;
+    const u32x4 ones = pack<T>(one);
+
+    if (begin < end) load(begin);
+    for (int64_t m0 = begin; m0 < end; m0 += MR) {
+        __syncthreads();
+        store(m0);
+        __syncthreads();
+        if (m0 + MR < end) load(m0 + MR);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            u32x4 fz[A], fx[B];
+#pragma unroll
+            for (int i = 0; i < A; ++i) fz[i] = read_transposed<T, false>(z_lds, PZ, c * KC, wn * A + i, lane);
+#pragma unroll
+            for (int j = 0; j < B; ++j) fx[j] = read_transposed<T, false>(x_lds, PX, c * KC, wk * B + j, lane);
+#pragma unroll
+            for (int i = 0; i < A; ++i)
+#pragma unroll
+                for (int j = 0; j < B; ++j) acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
+            if (sum_bias) {
+#pragma unroll
+                for (int i = 0; i < A; ++i) acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
+            }
+        }
+    }
+
+    float* part = a.part + split * ((int64_t)a.N * a.K + a.N);
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int n = n0 + (wn * A + i) * 16 + 4 * q + e;
+            if (n >= a.N) continue;
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                const int k = k0 + (wk * B + j) * 16 + r;
+                if (k < a.K) part[(int64_t)n * a.K + k] = acc[i][j][e];
+            }
+            if (sum_bias && r == 0) part[(int64_t)a.N * a.K + n] = acc_b[i][e];
+        }
+}
+
+// Sums over the splits, in a fixed order: a block takes 32 outputs, 8 lanes
+// each for every eighth split.  The first `weights` outputs are dW's, the rest db's.
+template <class T>
+__global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict__ part, int splits, int64_t weights,
+                                                         int64_t count, T* __restrict__ dw, T* __restrict__ db) {
+    __shared__ float lds[8][32];
+    const int col = threadIdx.x & 31, lane = threadIdx.x >> 5;
+    const int64_t i = (int64_t)blockIdx.x * 32 + col;
+    float total = 0.0f;
+    if (i < count) {
+#pragma unroll 8
+        for (int s = lane; s < splits; s += 8) total += part[(int64_t)s * count + i];
+    }
+    lds[lane][col] = total;
+    __syncthreads();
+    if (lane == 0 && i < count) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) total += lds[k][col];
+        if (i < weights) {
+            if (dw) dw[i] = (T)total;
+        } else if (db) {
+            db[i - weights] = (T)total;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+// Widths in powers of two: chunks of the contracted dimension, 16-column tiles.
+template <class T>
+static int chunks_of(int channels) {
+    const int chunks = (channels + CHUNK<T> - 1) / CHUNK<T>;
+    return chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : chunks <= 8 ? 8 : 16;
+}
+
+template <class T, bool Q8, int EPI, int KCH, int NT>
+static void launch_stream_as(LinearRows a, hipStream_t stream) {
+    a.n_tiles = (a.N + 16 * NT - 1) / (16 * NT);
+    // 512 rows a block at most, fewer where that would leave less than eight
+    // blocks a compute unit: a block reads its weights once.
+    int64_t strips = a.rows * a.n_tiles / (16 * 2048) / 4 * 4;
+    a.strips = (int)(strips < 4 ? 4 : strips > 32 ? 32 : strips);
+    const int64_t row_blocks = (a.rows + 16 * a.strips - 1) / (16 * a.strips);
+    const int64_t blocks = (row_blocks + 7) / 8 * 8 * a.n_tiles;
+    hipLaunchKernelGGL((linear_stream_kernel<T, Q8, EPI, KCH, NT>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+}
+template <class T, bool Q8, int EPI, int KCH>
+static void launch_stream(const LinearRows& a, hipStream_t stream) {
+    // Few rows: narrow column tiles, so that many compute units read the
+    // weights at once.
+    if (a.N <= 32 || a.rows <= 1024) launch_stream_as<T, Q8, EPI, KCH, 2>(a, stream);
+    else if (a.N <= 64) launch_stream_as<T, Q8, EPI, KCH, 4>(a, stream);
+    else launch_stream_as<T, Q8, EPI, KCH, 8>(a, stream);
+}
+
+template <class T, bool Q8, int EPI, int RS, int NT>
+static void launch_rows_as(LinearRows a, hipStream_t stream) {
+    a.n_tiles = (a.N + 16 * NT - 1) / (16 * NT);
+    const int64_t row_blocks = (a.rows + 64 * RS - 1) / (64 * RS);
+    const int64_t blocks = (row_blocks + 7) / 8 * 8 * a.n_tiles;
+    hipLaunchKernelGGL((linear_rows_kernel<T, Q8, EPI, RS, NT>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+}
+
+template <class T, bool Q8, int EPI>
+static void launch_rows(const LinearRows& a, hipStream_t stream) {
+    switch (chunks_of<T>(a.K)) {
+        case 1: return launch_stream<T, Q8, EPI, 1>(a, stream);
+        case 2: return launch_stream<T, Q8, EPI, 2>(a, stream);
+        case 4: return launch_stream<T, Q8, EPI, 4>(a, stream);
+        case 8: return launch_stream<T, Q8, EPI, 8>(a, stream);
+    }
+    if (a.N <= 32 || a.rows <= 1024) launch_rows_as<T, Q8, EPI, 1, 2>(a, stream);
+    else if (a.N <= 64) launch_rows_as<T, Q8, EPI, 2, 4>(a, stream);
+    else launch_rows_as<T, Q8, EPI, 2, 8>(a, stream);
+}
+
+template <class T, bool Q8, int A, int B>
+static void launch_gradw_as(const LinearGradW& a, int splits, hipStream_t stream) {
+    hipLaunchKernelGGL((linear_gradw_kernel<T, Q8, A, B>), dim3((unsigned)(a.n_tiles * a.k_tiles * splits)), dim3(256),
+                       0, stream, a);
+}
+template <class T, bool Q8, int A>
+static void launch_gradw_b(const LinearGradW& a, int splits, hipStream_t stream) {
+    if (a.K <= 32) launch_gradw_as<T, Q8, A, 1>(a, splits, stream);
+    else if (a.K <= 64) launch_gradw_as<T, Q8, A, 2>(a, splits, stream);
+    else launch_gradw_as<T, Q8, A, 4>(a, splits, stream);
+}
+template <class T, bool Q8>
+static void launch_gradw(const LinearGradW& a, int splits, hipStream_t stream) {
+    if (a.N <= 32) launch_gradw_b<T, Q8, 1>(a, splits, stream);
+    else if (a.N <= 64) launch_gradw_b<T, Q8, 2>(a, splits, stream);
+    else launch_gradw_b<T, Q8, 4>(a, splits, stream);
+}
+
+// How the rows of a backward pass are split: the fused kernel's blocks, or the
+// weight gradient's splits.
+struct BwdPlan {
+    bool fused;
+    int splits, n_tiles, k_tiles;
+    int64_t rows_per_split;
+};
+static int gradw_tiles(int n) { return n <= 32 ? 1 : n <= 64 ? 1 : (n + 127) / 128; }
+template <class T>
+static BwdPlan bwd_plan(int64_t rows, int K, int N) {
+    BwdPlan p;
+    p.fused = fused_fits<T>(K, N);
+    p.n_tiles = p.fused ? 1 : gradw_tiles(N);
+    p.k_tiles = p.fused ? 1 : gradw_tiles(K);
+    // Two blocks per compute unit in all, and 64 rows a block at least.
+    int64_t splits = 512 / (p.n_tiles * p.k_tiles);
+    const int64_t most = (rows + 63) / 64;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    p.rows_per_split = ((rows + splits - 1) / splits + 63) / 64 * 64;
+    if (p.rows_per_split < 64) p.rows_per_split = 64;
+    p.splits = (int)((rows + p.rows_per_split - 1) / p.rows_per_split);
+    if (p.splits < 1) p.splits = 1;
+    return p;
+}
+
+static size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// Scratch of the backward pass: the splits' dW and db; unless it is fused also
+// dz and W^T.
+struct BwdScratch {
+    size_t part, dz, wt, total;
+};
+template <class T>
+static BwdScratch bwd_scratch(int64_t rows, int K, int N) {
+    const BwdPlan p = bwd_plan<T>(rows, K, N);
+    BwdScratch s;
+    s.part = 0;
+    s.dz = aligned((size_t)p.splits * ((size_t)N * K + N) * 4);
+    s.wt = s.dz + (p.fused ? 0 : aligned((size_t)rows * N * sizeof(T)));
+    s.total = s.wt + (p.fused ? 0 : aligned((size_t)N * K * sizeof(T)));
+    return s;
+}
+
+template <class T>
+static int linear_fwd(const gs3d_linear_args& g, hipStream_t stream) {
+    LinearRows a{};
+    a.x = Rows{g.x, g.x_stride, {}, g.inner};
+    a.w = g.weight, a.bias = g.bias, a.other = g.residual, a.ldo = g.residual_stride, a.y = g.y;
+    a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
+    launch_rows<T, false, 0>(a, stream);
+    return launch_status("gs3d_linear_fwd");
+}
+
+template <class T, bool Q8>
+static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t stream) {
+    const BwdPlan p = bwd_plan<T>(g.rows, g.inner, g.outer);
+    const BwdScratch at = bwd_scratch<T>(g.rows, g.inner, g.outer);
+    // Without an activation only dW sees the input: no channels otherwise.
+    const int seen = g.grad_weight || g.activation != GS3D_ACT_NONE ? g.inner : 0;
+    const Rows x{g.x, g.x_stride, {g.codes, g.scales, seen}, seen};
+    const bool params = g.grad_weight || g.grad_bias;
+    float* part = reinterpret_cast<float*>(scratch + at.part);
+    if (p.fused) {
+        if (g.rows > 0 || params) {
+            LinearFused a{x, g.weight, g.bias, g.upstream, g.upstream_stride, g.grad_x, params ? part : nullptr,
+                          g.rows, p.rows_per_split, g.inner, g.outer, g.activation};
+            fused_launch<T>(a, Q8, p.splits, stream);
+        }
+    } else {
+        const void* dz = g.upstream;
+        int64_t ldz = g.upstream_stride;
+        if (g.activation != GS3D_ACT_NONE && g.rows > 0) {
+            LinearRows a{};
+            a.x = x, a.w = g.weight, a.bias = g.bias, a.other = g.upstream, a.ldo = g.upstream_stride;
+            a.y = scratch + at.dz;
+            a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
+            launch_rows<T, Q8, 1>(a, stream);
+            dz = scratch + at.dz;
+            ldz = g.outer;
+        }
+        if (g.grad_x && g.rows > 0) {
+            T* wt = reinterpret_cast<T*>(scratch + at.wt);
+            hipLaunchKernelGGL(transpose_kernel<T>, dim3((g.inner + 31) / 32, (g.outer + 31) / 32), dim3(256), 0,
+                               stream, static_cast<const T*>(g.weight), g.outer, g.inner, wt);
+            LinearRows a{};
+            a.x = Rows{dz, ldz, {}, g.outer}, a.w = wt, a.y = g.grad_x;
+            a.rows = g.rows, a.K = g.outer, a.N = g.inner, a.act = GS3D_ACT_NONE;
+            launch_rows<T, false, 0>(a, stream);
+        }
+        if (params) {
+            LinearGradW a{x, dz, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, part, g.inner};
+            launch_gradw<T, Q8>(a, p.splits, stream);
+        }
+    }
+    if (params) {
+        const int64_t weights = (int64_t)g.outer * g.inner, count = weights + g.outer;
+        hipLaunchKernelGGL(sum_splits_kernel<T>, dim3(blocks_for(count, 32)), dim3(256), 0, stream, part, p.splits,
+                           weights, count, static_cast<T*>(g.grad_weight), static_cast<T*>(g.grad_bias));
+    }
+    return launch_status("gs3d_linear_bwd");
+}
+
+}  // namespace gs3d

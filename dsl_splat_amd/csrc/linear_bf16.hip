@@ -1,0 +1,14 @@
+// Per-pixel products (linear.hpp) for bf16.
+#include "linear.hpp"
+
+namespace gs3d {
+
+int linear_fwd_bf16(const gs3d_linear_args& g, hipStream_t stream) { return linear_fwd<bf16_t>(g, stream); }
+
+int linear_bwd_bf16(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t stream) {
+    return g.codes ? linear_bwd<bf16_t, true>(g, scratch, stream) : linear_bwd<bf16_t, false>(g, scratch, stream);
+}
+
+size_t linear_bwd_bytes_bf16(int64_t rows, int K, int N) { return bwd_scratch<bf16_t>(rows, K, N).total; }
+
+}  // namespace gs3d
