@@ -389,6 +389,26 @@ GS3D_DEV f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
     }
 }
 
+// multiply() for a chunk of which only the first `valid` elements count (the
+// rest are zero), `valid` the same in the whole wavefront.  Float skips the
+// instructions that would contract zeros only: matrix instructions bound its
+// products, and 33 channels are then 36 and not 48.
+template <class T>
+GS3D_DEV f32x4 multiply_chunk(u32x4 a, u32x4 b, f32x4 c, int valid) {
+    if constexpr (sizeof(T) == 4) {
+        if (valid <= 0) return c;
+        if (valid < 4) {
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[0]), __uint_as_float(b[0]), c, 0, 0, 0);
+            if (valid > 1)
+                c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[1]), __uint_as_float(b[1]), c, 0, 0, 0);
+            if (valid > 2)
+                c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[2]), __uint_as_float(b[2]), c, 0, 0, 0);
+            return c;
+        }
+    }
+    return multiply<T>(a, b, c);
+}
+
 // Column of row r of tile t in an operand whose rows become an output's
 // columns.  A lane ends up with rows 4q..4q+3 of every tile; for 16-bit types
 // two tiles are dealt out so that their eight values are neighbours, 16 bytes

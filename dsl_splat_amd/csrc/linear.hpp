@@ -4,7 +4,7 @@
 //
 //   linear_stream_kernel     rows times weights that lie in LDS whole, while the
 //                            rows stream past: every product whose contracted
-//                            dimension has at most 8 chunks
+//                            dimension has at most 4 chunks
 //   linear_rows_kernel       the same for longer ones, the weights in steps
 //   linear_bwd_fused_kernel  the whole backward pass in one (linear_fused.hpp),
 //                            where its weights and their gradient fit a block
@@ -64,9 +64,9 @@ GS3D_DEV u32x4 linear_end(const LinearRows& a, float (&z)[E], u32x4 raw_other) {
 // Wavefronts a SIMD that the stream kernel's registers leave room for.
 template <class T, bool Q8, int KCH, int NT>
 constexpr int stream_waves() {
-    if (sizeof(T) == 4) return KCH == 8 ? (NT == 8 ? 1 : 2) : KCH == 4 ? (NT == 8 ? 2 : 3) : NT == 8 ? 3 : 4;
-    if (Q8) return KCH == 8 ? 1 : KCH == 4 ? (NT == 8 ? 2 : 3) : 4;
-    return KCH == 8 ? 2 : NT == 8 ? 4 : 5 - (KCH == 4 ? 1 : 0);
+    if (sizeof(T) == 4) return KCH == 4 ? (NT == 8 ? 2 : 3) : NT == 8 ? 3 : 4;
+    if (Q8) return KCH == 4 ? (NT == 8 ? 2 : 3) : 4;
+    return NT == 8 || KCH == 4 ? 4 : 5;
 }
 
 // A block of 4 wavefronts holds the weights of 16 NT columns in LDS, in
@@ -134,6 +134,7 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, KCH, NT>())) void linear_
         asm volatile("" : "+v"(mine));
 #pragma unroll
         for (int g = 0; g < G; ++g) {
+            if (sizeof(T) == 4 && n0 + g * KC >= a.N) break;
             f32x4 acc[TG];
 #pragma unroll
             for (int t = 0; t < TG; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, KCH, NT>())) void linear_
             for (int c = 0; c < KCH; ++c)
 #pragma unroll
                 for (int t = 0; t < TG; ++t)
-                    acc[t] = multiply<T>(w_lds[(c * NT + g * TG + t) * 64 + mine], xf[c], acc[t]);
+                    acc[t] = multiply_chunk<T>(w_lds[(c * NT + g * TG + t) * 64 + mine], xf[c], acc[t], a.K - c * KC);
             const int at = g * KC + q * E;
             float z[E];
 #pragma unroll
@@ -154,17 +155,22 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, KCH, NT>())) void linear_
     }
 }
 
-// Longer contracted dimensions: a block of 4 wavefronts computes 64 RS rows x
-// 16 NT columns, the weights' fragments of CH chunks at a time through LDS for
-// all four, the next step's operands loaded while this one's are multiplied.
+// Longer contracted dimensions, where the products count more than the bytes:
+// a block of 4 wavefronts computes 64 RS rows x 16 NT columns.  CH chunks of
+// the weights at a time go through LDS, twice buffered, so a step has one
+// barrier; a fragment read from there serves the RS strips of a wavefront
+// (the LDS port, 128 bytes a clock, would bound RS = 1: 8 clocks a fragment
+// and wavefront, 16 clocks a matrix instruction).  The next step's operands
+// are loaded while this one's are multiplied.
 template <class T, bool Q8, int EPI, int RS, int NT>
-__global__ __launch_bounds__(256) void linear_rows_kernel(LinearRows a) {
+__global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
-    constexpr int CH = 2;            // chunks of the contracted dimension a step
-    constexpr int WL = CH * NT / 4;  // fragments of W a thread brings in
+    constexpr int CH = 2;                  // chunks of the contracted dimension a step
+    constexpr int WL = (CH * NT + 3) / 4;  // fragment vectors of W a thread brings in
     constexpr int TG = KC / 16;
-    __shared__ u32x4 w_lds[CH * NT * 64];
+    constexpr int G = NT / TG;
+    __shared__ u32x4 w_lds[2][CH * NT * 64];
     __shared__ float bias_lds[16 * NT];
 
     int64_t row_block;
@@ -203,6 +209,16 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(LinearRows a) {
 #pragma unroll
             for (int s = 0; s < RS; ++s) xr[s][c].issue(a.x, row[s], k0 + c * KC + q * E);
     };
+    auto store = [&](int k0, int buffer) {
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+            const int slot = i * 256 + tid;
+            if (CH * NT % 4 != 0 && slot >= CH * NT * 64) break;
+            const int c = slot / (NT * 64), t = (slot / 64) % NT, l = slot & 63;
+            const u32x4 v = finish_row<T>(wr[i], k0 + c * KC + (l >> 4) * E, a.K);
+            w_lds[buffer][slot] = n0 + tile_column<T>(t, l & 15) < a.N ? v : u32x4{0u, 0u, 0u, 0u};
+        }
+    };
 
     f32x4 acc[RS][NT];
 #pragma unroll
@@ -211,30 +227,27 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(LinearRows a) {
         for (int t = 0; t < NT; ++t) acc[s][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     load(0);
+    store(0, 0);
+    int buffer = 0;
     for (int k0 = 0; k0 < a.K; k0 += CH * KC) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < WL; ++i) {
-            const int slot = i * 256 + tid;
-            const int c = slot / (NT * 64), t = (slot / 64) % NT, l = slot & 63;
-            const u32x4 v = finish_row<T>(wr[i], k0 + c * KC + (l >> 4) * E, a.K);
-            w_lds[slot] = n0 + tile_column<T>(t, l & 15) < a.N ? v : u32x4{0u, 0u, 0u, 0u};
-        }
         u32x4 xc[RS][CH];
 #pragma unroll
         for (int s = 0; s < RS; ++s)
 #pragma unroll
             for (int c = 0; c < CH; ++c) xc[s][c] = xr[s][c].finish(a.x, k0 + c * KC + q * E);
         __syncthreads();
-        if (k0 + CH * KC < a.K) load(k0 + CH * KC);
+        const bool more = k0 + CH * KC < a.K;
+        if (more) load(k0 + CH * KC);
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const u32x4 wf = w_lds[(c * NT + t) * 64 + lane];
+                const u32x4 wf = w_lds[buffer][(c * NT + t) * 64 + lane];
 #pragma unroll
                 for (int s = 0; s < RS; ++s) acc[s][t] = multiply<T>(wf, xc[s][c], acc[s][t]);
             }
+        buffer ^= 1;
+        if (more) store(k0 + CH * KC, buffer);
     }
 
     T* y = static_cast<T*>(a.y);
@@ -243,15 +256,20 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(LinearRows a) {
     for (int s = 0; s < RS; ++s) {
         const int64_t m = first + wave * (16 * RS) + 16 * s + r;
         if (m >= a.rows) continue;
+        u32x4 o[G];
+        if (EPI == 1 || other) {
 #pragma unroll
-        for (int g = 0; g < NT / TG; ++g) {
+            for (int g = 0; g < G; ++g) o[g] = issue_row(other + m * a.ldo, n0 + g * KC + q * E, a.N);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
             const int at = g * KC + q * E;  // column within the block's tile
             if (n0 + at >= a.N) continue;
             float z[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) z[i] = acc[s][g * TG + i / 4][i & 3] + bias_lds[at + i];
             u32x4 raw = {0u, 0u, 0u, 0u};
-            if (EPI == 1 || other) raw = load_row(other + m * a.ldo, n0 + at, a.N);
+            if (EPI == 1 || other) raw = finish_row<T>(o[g], n0 + at, a.N);
             store_row(y + m * a.N, n0 + at, a.N, linear_end<T, EPI, E>(a, z, raw));
         }
     }
@@ -429,7 +447,7 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict
 template <class T>
 static int chunks_of(int channels) {
     const int chunks = (channels + CHUNK<T> - 1) / CHUNK<T>;
-    return chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : chunks <= 8 ? 8 : 16;
+    return chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : 8;
 }
 
 template <class T, bool Q8, int EPI, int KCH, int NT>
@@ -466,11 +484,11 @@ static void launch_rows(const LinearRows& a, hipStream_t stream) {
         case 1: return launch_stream<T, Q8, EPI, 1>(a, stream);
         case 2: return launch_stream<T, Q8, EPI, 2>(a, stream);
         case 4: return launch_stream<T, Q8, EPI, 4>(a, stream);
-        case 8: return launch_stream<T, Q8, EPI, 8>(a, stream);
     }
-    if (a.N <= 32 || a.rows <= 1024) launch_rows_as<T, Q8, EPI, 1, 2>(a, stream);
-    else if (a.N <= 64) launch_rows_as<T, Q8, EPI, 2, 4>(a, stream);
-    else launch_rows_as<T, Q8, EPI, 2, 8>(a, stream);
+    if (a.rows <= 1024) launch_rows_as<T, Q8, EPI, 1, 2>(a, stream);
+    else if (a.N <= 32) launch_rows_as<T, Q8, EPI, 4, 2>(a, stream);
+    else if (a.N <= 64) launch_rows_as<T, Q8, EPI, 4, 4>(a, stream);
+    else launch_rows_as<T, Q8, EPI, 4, 8>(a, stream);
 }
 
 template <class T, bool Q8, int A, int B>

@@ -42,6 +42,12 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
     constexpr int KC = CHUNK<T>;
     constexpr int TG = KC / 16;              // tiles a chunk
     constexpr int KT = KCH * TG, NT = NCH * TG;
+    // dW's tiles over the wavefronts: 2 x 2, or for float, whose matrix
+    // instructions count most and skip what lies past K or N, N's dealt to all
+    // four (33 x 97: at most 2 x 3 tiles a wavefront, not 4 x 2).
+    constexpr int WN = sizeof(T) == 4 && NT >= 4 ? 4 : 2, WK = 4 / WN;
+    constexpr int TN = NT / WN, TK = KT / WK;
+    constexpr bool SKIP = sizeof(T) == 4;
     constexpr int PK = KCH * 4 + 1, PN = NCH * 4 + 1;  // pitches: the odd unit spreads rows over the banks
     __shared__ u32x4 w_lds[NCH * KC * PK];
     __shared__ u32x4 x_lds[64 * PK];
@@ -50,7 +56,7 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, q = lane >> 4;
-    const int wn = wave >> 1, wk = wave & 1;
+    const int wn = wave / WK, wk = wave % WK;
     const int64_t begin = blockIdx.x * a.rows_per_block;
     const int64_t end = begin + a.rows_per_block < a.rows ? begin + a.rows_per_block : a.rows;
     const T* w = static_cast<const T*>(a.w);
@@ -71,12 +77,12 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
         return m < end ? m : end - 1;
     };
 
-    f32x4 acc[NT / 2][KT / 2], acc_b[NT / 2];
+    f32x4 acc[TN][TK], acc_b[TN];
 #pragma unroll
-    for (int i = 0; i < NT / 2; ++i) {
+    for (int i = 0; i < TN; ++i) {
         acc_b[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < KT / 2; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < TK; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     float one[E];
 #pragma unroll
@@ -113,6 +119,7 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
         for (int t = 0; t < KT; ++t) out[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int g = 0; g < NCH; ++g) {
+            if (SKIP && g * KC >= a.N) break;
             u32x4 dz = finish_row<T>(yr[g], g * KC + q * E, a.N);
             yr[g] = issue_row(dy + next * a.ldy, g * KC + q * E, a.N);
             if (a.act != GS3D_ACT_NONE) {
@@ -123,7 +130,8 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
                 for (int c = 0; c < KCH; ++c)
 #pragma unroll
                     for (int t = 0; t < TG; ++t)
-                        z[t] = multiply<T>(w_lds[tile_column<T>(g * TG + t, r) * PK + c * 4 + q], xf[c], z[t]);
+                        z[t] = multiply_chunk<T>(w_lds[tile_column<T>(g * TG + t, r) * PK + c * 4 + q], xf[c], z[t],
+                                                 a.K - c * KC);
                 float arg[E], grad[E];
                 unpack<T>(dz, grad);
 #pragma unroll
@@ -135,8 +143,11 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
             if (a.part) z_lds[(wave * 16 + r) * PN + g * 4 + q] = dz;
             if (dx) {
 #pragma unroll
-                for (int t = 0; t < KT; ++t)
-                    out[t] = multiply<T>(read_transposed<T, true>(w_lds, PK, g * KC, t, lane), dz, out[t]);
+                for (int t = 0; t < KT; ++t) {
+                    if (SKIP && t * 16 >= a.K) break;
+                    out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, t, lane), dz, out[t],
+                                               a.N - g * KC);
+                }
             }
         }
         if (dx && valid) {
@@ -152,20 +163,20 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
             __syncthreads();
 #pragma unroll
             for (int c = 0; c < 64 / KC; ++c) {
-                u32x4 fz[NT / 2], fx[KT / 2];
+                u32x4 fz[TN], fx[TK];
 #pragma unroll
-                for (int i = 0; i < NT / 2; ++i)
-                    fz[i] = read_transposed<T, false>(z_lds, PN, c * KC, wn * (NT / 2) + i, lane);
+                for (int i = 0; i < TN; ++i) fz[i] = read_transposed<T, false>(z_lds, PN, c * KC, i * WN + wn, lane);
 #pragma unroll
-                for (int j = 0; j < KT / 2; ++j)
-                    fx[j] = read_transposed<T, false>(x_lds, PK, c * KC, wk * (KT / 2) + j, lane);
+                for (int j = 0; j < TK; ++j) fx[j] = read_transposed<T, false>(x_lds, PK, c * KC, j * WK + wk, lane);
 #pragma unroll
-                for (int i = 0; i < NT / 2; ++i)
+                for (int i = 0; i < TN; ++i) {
+                    if (SKIP && (i * WN + wn) * 16 >= a.N) break;
 #pragma unroll
-                    for (int j = 0; j < KT / 2; ++j) acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
-                if (wk == 0) {
-#pragma unroll
-                    for (int i = 0; i < NT / 2; ++i) acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
+                    for (int j = 0; j < TK; ++j) {
+                        if (SKIP && (j * WK + wk) * 16 >= a.K) break;
+                        acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
+                    }
+                    if (wk == 0) acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
                 }
             }
         }
@@ -174,14 +185,14 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
     if (!a.part) return;
     float* part = a.part + (int64_t)blockIdx.x * ((int64_t)a.N * a.K + a.N);
 #pragma unroll
-    for (int i = 0; i < NT / 2; ++i)
+    for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int n = (wn * (NT / 2) + i) * 16 + 4 * q + e;
+            const int n = (i * WN + wn) * 16 + 4 * q + e;
             if (n >= a.N) continue;
 #pragma unroll
-            for (int j = 0; j < KT / 2; ++j) {
-                const int k = (wk * (KT / 2) + j) * 16 + r;
+            for (int j = 0; j < TK; ++j) {
+                const int k = (j * WK + wk) * 16 + r;
                 if (k < a.K) part[(int64_t)n * a.K + k] = acc[i][j][e];
             }
             if (wk == 0 && r == 0) part[(int64_t)a.N * a.K + n] = acc_b[i][e];
