@@ -95,7 +95,7 @@ GS3D_DEV u32x4 pack(const float (&v)[8]) {
 // it, finish_row makes the elements past the row's end zero.  A vector that
 // would reach past the end is read from the row's last VEC<T> elements and
 // shifted down, so nothing beyond the row is read.  Rows shorter than a
-// vector are read element by element; a row of no channels is not read.
+// vector are read element by element.
 template <int UNIT_BITS>
 GS3D_DEV u32x4 shift_down(u32x4 raw, int units) {
     if (units * UNIT_BITS >= 128) return u32x4{0u, 0u, 0u, 0u};
@@ -107,12 +107,13 @@ GS3D_DEV u32x4 shift_down(u32x4 raw, int units) {
     return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
 
-template <class T>
+// WIDE promises rows of at least a vector: no branch at all then, so that the
+// compiler can count the loads in flight exactly.
+template <class T, bool WIDE = false>
 GS3D_DEV u32x4 issue_row(const T* row, int at, int count) {
     constexpr int E = VEC<T>;
-    if (count >= E) return load16(row + (at < count - E ? at : count - E));
+    if (WIDE || count >= E) return load16(row + (at < count - E ? at : count - E));
     u32x4 raw = {0u, 0u, 0u, 0u};
-    if (count <= 0) return raw;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const int k = at + i < count ? at + i : count - 1;
@@ -126,12 +127,19 @@ GS3D_DEV u32x4 issue_row(const T* row, int at, int count) {
     }
     return raw;
 }
-template <class T>
+template <class T, bool WIDE = false>
 GS3D_DEV u32x4 finish_row(u32x4 raw, int at, int count) {
     constexpr int E = VEC<T>;
     const int over = at + E - count;
-    if (count >= E && over > 0) return shift_down<8 * (int)sizeof(T)>(raw, over);
+    if ((WIDE || count >= E) && over > 0) return shift_down<8 * (int)sizeof(T)>(raw, over);
     return raw;
+}
+// finish_row for the wavefront's vectors of one chunk, from `first` on: looked
+// at only where the chunk (a scalar) reaches past the row.
+template <class T, bool WIDE>
+GS3D_DEV u32x4 finish_chunk(u32x4 raw, int first, int at, int count) {
+    if (first + 4 * VEC<T> <= count) return raw;
+    return finish_row<T, WIDE>(raw, at, count);
 }
 template <class T>
 GS3D_DEV u32x4 load_row(const T* row, int at, int count) {
@@ -290,15 +298,14 @@ struct Q8Raw {
     uint32_t scale;
 };
 
-template <class T>
+template <class T, bool WIDE = false>
 GS3D_DEV Q8Raw issue_row_q8(const Q8Rows& q, int64_t row, int at) {
     constexpr int E = VEC<T>;
     const int8_t* p = q.codes + row * q.channels;
     Q8Raw raw = {0u, 0u};
-    if (q.channels <= 0) return raw;
     const int block = (at < q.channels ? at : q.channels - 1) >> 5;
     raw.scale = q.scales[row * ((q.channels + 31) >> 5) + block];
-    if (q.channels >= E) {
+    if (WIDE || q.channels >= E) {
         p += at < q.channels - E ? at : q.channels - E;
         if constexpr (E == 8) {
             const u32x2 w = *reinterpret_cast<const u32x2_at1*>(p);
@@ -307,7 +314,6 @@ GS3D_DEV Q8Raw issue_row_q8(const Q8Rows& q, int64_t row, int at) {
             raw.codes = *reinterpret_cast<const u32_at1*>(p);
         }
     } else {
-        raw.codes = 0u;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const uint32_t v = (uint8_t)p[at + i < q.channels ? at + i : q.channels - 1];
@@ -318,17 +324,18 @@ GS3D_DEV Q8Raw issue_row_q8(const Q8Rows& q, int64_t row, int at) {
 }
 
 // An element past the row's end is zero also where the row ends in a block
-// that reads back as NaN.
-template <class T>
-GS3D_DEV u32x4 finish_row_q8(Q8Raw raw, int at, int channels) {
+// that reads back as NaN.  `inside`: the caller knows that no lane reaches
+// past the end.
+template <class T, bool WIDE = false>
+GS3D_DEV u32x4 finish_row_q8(Q8Raw raw, int at, int channels, bool inside = false) {
     constexpr int E = VEC<T>;
     const int over = at + E - channels;
-    if (channels >= E && over > 0) raw.codes = over >= E ? 0u : raw.codes >> (8 * over);
+    if (!inside && (WIDE || channels >= E) && over > 0) raw.codes = over >= E ? 0u : raw.codes >> (8 * over);
     const float scale = q8_scale(raw.scale);
     float v[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) v[i] = (float)(int)(int8_t)(raw.codes >> (8 * i)) * scale;
-    if (over > 0) {
+    if (!inside && over > 0) {
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] = at + i < channels ? v[i] : 0.0f;
     }
@@ -346,20 +353,33 @@ struct Rows {
     Q8Rows q8;
     int channels;
 };
-template <class T, bool Q8>
+template <class T, bool Q8, bool WIDE = false>
 struct RowRaw {
     u32x4 raw;
     GS3D_DEV void issue(const Rows& a, int64_t row, int at) {
-        raw = issue_row(static_cast<const T*>(a.x) + row * a.ldx, at, a.channels);
+        raw = issue_row<T, WIDE>(static_cast<const T*>(a.x) + row * a.ldx, at, a.channels);
     }
-    GS3D_DEV u32x4 finish(const Rows& a, int at) const { return finish_row<T>(raw, at, a.channels); }
+    GS3D_DEV u32x4 finish(const Rows& a, int at) const { return finish_row<T, WIDE>(raw, at, a.channels); }
+    GS3D_DEV u32x4 finish_in(const Rows& a, int first, int at) const {
+        return finish_chunk<T, WIDE>(raw, first, at, a.channels);
+    }
 };
-template <class T>
-struct RowRaw<T, true> {
+template <class T, bool WIDE>
+struct RowRaw<T, true, WIDE> {
     Q8Raw raw;
-    GS3D_DEV void issue(const Rows& a, int64_t row, int at) { raw = issue_row_q8<T>(a.q8, row, at); }
-    GS3D_DEV u32x4 finish(const Rows& a, int at) const { return finish_row_q8<T>(raw, at, a.channels); }
+    GS3D_DEV void issue(const Rows& a, int64_t row, int at) { raw = issue_row_q8<T, WIDE>(a.q8, row, at); }
+    GS3D_DEV u32x4 finish(const Rows& a, int at) const { return finish_row_q8<T, WIDE>(raw, at, a.channels); }
+    GS3D_DEV u32x4 finish_in(const Rows& a, int first, int at) const {
+        return finish_row_q8<T, WIDE>(raw, at, a.channels, first + 4 * VEC<T> <= a.channels);
+    }
 };
+
+// store_row for the wavefront's vectors of one chunk from `first` on.
+template <class T>
+GS3D_DEV void store_chunk(T* row, int first, int at, int count, u32x4 raw) {
+    if (first + 4 * VEC<T> <= count) store16(row + at, raw);
+    else store_row(row, at, count, raw);
+}
 
 // ---------------------------------------------------------------------------
 // Matrix fragments.  A fragment is 16 bytes a lane: lane l holds row l % 16

@@ -12,8 +12,9 @@
 //                            the rows, after dz and dx from the kernels above
 //   sum_splits_kernel        the blocks' partial sums in a fixed order
 //
-// The products of the forward (EPI 0) end in act and r; those of the backward
-// (EPI 1) in dz = dy act'(x W^T + b), z computed again rather than kept.
+// The products of the forward end in act (EPI 0), or in act and + r (EPI 2);
+// those of the backward (EPI 1) in dz = dy act'(x W^T + b), z computed again
+// rather than kept.
 // Products of 16-bit types go through matrix instructions with sums in 32
 // bits.  dz is rounded to the element type once, as the operand of the two
 // products that follow it.
@@ -27,7 +28,7 @@ struct LinearRows {
     Rows x;              // rows x K
     const void* w;       // N x K
     const void* bias;    // N or NULL
-    const void* other;   // EPI 0: residual or NULL; EPI 1: dy
+    const void* other;   // EPI 1: dy; EPI 2: residual
     int64_t ldo;
     void* y;             // rows x N
     int64_t rows;
@@ -46,14 +47,13 @@ GS3D_DEV void xcd_block(const LinearRows& a, int64_t& row_block, int& n_tile) {
 template <class T, int EPI, int E>
 GS3D_DEV u32x4 linear_end(const LinearRows& a, float (&z)[E], u32x4 raw_other) {
     float o[E];
+    if constexpr (EPI != 0) unpack<T>(raw_other, o);
     if constexpr (EPI == 1) {
-        unpack<T>(raw_other, o);
         pull_back(o, z, a.act);
         return pack<T>(o);
     } else {
         activate(z, a.act);
-        if (a.other) {
-            unpack<T>(raw_other, o);
+        if constexpr (EPI == 2) {
 #pragma unroll
             for (int i = 0; i < E; ++i) z[i] += o[i];
         }
@@ -62,11 +62,11 @@ GS3D_DEV u32x4 linear_end(const LinearRows& a, float (&z)[E], u32x4 raw_other) {
 }
 
 // Wavefronts a SIMD that the stream kernel's registers leave room for.
-template <class T, bool Q8, int KCH, int NT>
+template <class T, bool Q8, int EPI, int KCH, int NT>
 constexpr int stream_waves() {
-    if (sizeof(T) == 4) return KCH == 4 ? (NT == 8 ? 2 : 3) : NT == 8 ? 3 : 4;
-    if (Q8) return KCH == 4 ? (NT == 8 ? 2 : 3) : 4;
-    return NT == 8 || KCH == 4 ? 4 : 5;
+    const int wide = sizeof(T) == 4 ? 2 : 1;  // float holds twice the vectors
+    const int vectors = wide * (2 * KCH + (EPI != 0 ? NT / 2 : 0));
+    return vectors <= 4 ? 6 : vectors <= 8 ? 5 : vectors <= 12 ? 4 : vectors <= 16 ? 3 : 2;
 }
 
 // A block of 4 wavefronts holds the weights of 16 NT columns in LDS, in
@@ -75,15 +75,23 @@ constexpr int stream_waves() {
 // reads its strip straight into fragments, 64 bytes of a row at a time, the
 // next strip while this one is multiplied; the wavefronts never wait for one
 // another.  W's rows are the first operand, so a lane ends with 16 bytes of
-// one output row.  HBM bounds it while K and N are small.
-template <class T, bool Q8, int EPI, int KCH, int NT>
-__global__ __launch_bounds__(256, (stream_waves<T, Q8, KCH, NT>())) void linear_stream_kernel(LinearRows a) {
+// one output row; the sums start at the bias.  HBM bounds it while K and N are
+// small.
+//
+// Loads wait for the stores issued before them, so the next strip's are issued
+// first, and whole strips store without a branch: the wait for a load then
+// leaves the stores after it in flight.
+template <class T, bool Q8, int EPI, int KCH, int NT, bool WIDE>
+__global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void linear_stream_kernel(LinearRows a) {
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
     constexpr int TG = KC / 16;  // tiles of a lane's 16-byte output vector
     constexpr int G = NT / TG;
+    constexpr int VP = 16 * NT / E;  // vectors of a full output row
+    constexpr int PO = VP + 1;       // pitch of an output row in LDS
     __shared__ u32x4 w_lds[KCH * NT * 64];
-    __shared__ float bias_lds[16 * NT];
+    __shared__ u32x4 out_lds[4][16 * PO];
+    __shared__ f32x4 bias_lds[4 * NT];
 
     int64_t row_block;
     int n_tile;
@@ -107,27 +115,26 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, KCH, NT>())) void linear_
         w_lds[slot] = n < a.N ? load_row(w + (int64_t)n * a.K, k, a.K) : u32x4{0u, 0u, 0u, 0u};
     }
     if (tid < 16 * NT)
-        bias_lds[tid] = a.bias && n0 + tid < a.N ? to_f32(static_cast<const T*>(a.bias)[n0 + tid]) : 0.0f;
+        reinterpret_cast<float*>(bias_lds)[tid] =
+            a.bias && n0 + tid < a.N ? to_f32(static_cast<const T*>(a.bias)[n0 + tid]) : 0.0f;
     __syncthreads();
 
-    RowRaw<T, Q8> xr[KCH];
+    RowRaw<T, Q8, WIDE> xr[KCH];
     auto load = [&](int64_t m) {
         m = m < end ? m : end - 1;  // rows past the end repeat the last one and are not stored
 #pragma unroll
         for (int c = 0; c < KCH; ++c) xr[c].issue(a.x, m, c * KC + q * E);
     };
-    int64_t m = first + wave * 16 + r;
-    load(m);
-    for (; m - r < end; m += 64) {
+    auto strip = [&](int64_t m, auto whole) {
         u32x4 xf[KCH], o[G];
 #pragma unroll
-        for (int c = 0; c < KCH; ++c) xf[c] = xr[c].finish(a.x, c * KC + q * E);
-        if (EPI == 1 || other) {
-            const int64_t at = m < end ? m : end - 1;
+        for (int c = 0; c < KCH; ++c) xf[c] = xr[c].finish_in(a.x, c * KC, c * KC + q * E);
+        if constexpr (EPI != 0) {
+            const T* row = other + (whole.value || m < end ? m : end - 1) * a.ldo;
 #pragma unroll
-            for (int g = 0; g < G; ++g) o[g] = issue_row(other + at * a.ldo, n0 + g * KC + q * E, a.N);
+            for (int g = 0; g < G; ++g) o[g] = issue_row<T, WIDE>(row, n0 + g * KC + q * E, a.N);
         }
-        if (m - r + 64 < end) load(m + 64);
+        if constexpr (whole.value) load(m + 64);
         // The weights stay in LDS: hoisted out of the loop they would take
         // every register (128 at 4 chunks x 8 tiles).
         int mine = lane;
@@ -137,22 +144,40 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, KCH, NT>())) void linear_
             if (sizeof(T) == 4 && n0 + g * KC >= a.N) break;
             f32x4 acc[TG];
 #pragma unroll
-            for (int t = 0; t < TG; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < TG; ++t) acc[t] = bias_lds[g * 4 * TG + (mine >> 4) * TG + t];
 #pragma unroll
             for (int c = 0; c < KCH; ++c)
 #pragma unroll
                 for (int t = 0; t < TG; ++t)
                     acc[t] = multiply_chunk<T>(w_lds[(c * NT + g * TG + t) * 64 + mine], xf[c], acc[t], a.K - c * KC);
-            const int at = g * KC + q * E;
+            const int at = n0 + g * KC;
             float z[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) z[i] = acc[i / 4][i & 3] + bias_lds[at + i];
+            for (int i = 0; i < E; ++i) z[i] = acc[i / 4][i & 3];
             u32x4 raw = {0u, 0u, 0u, 0u};
-            if (EPI == 1 || other) raw = finish_row<T>(o[g], n0 + at, a.N);
-            raw = linear_end<T, EPI, E>(a, z, raw);
-            if (m < end) store_row(y + m * a.N, n0 + at, a.N, raw);
+            if constexpr (EPI != 0) raw = finish_chunk<T, WIDE>(o[g], at, at + q * E, a.N);
+            out_lds[wave][r * PO + g * 4 + q] = linear_end<T, EPI, E>(a, z, raw);
         }
-    }
+        // The strip's outputs leave in whole row segments: as they come, an
+        // instruction would write 64 bytes of 16 rows.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int vec = lane % VP, at = n0 + vec * E;
+#pragma unroll
+        for (int i = 0; i < 16 * VP / 64; ++i) {
+            const int row = i * (64 / VP) + lane / VP;
+            const u32x4 raw = out_lds[wave][row * PO + vec];
+            const int64_t to = m - r + row;
+            if (whole.value && n0 + 16 * NT <= a.N) store16(y + to * a.N + at, raw);
+            else if (to < end) store_row(y + to * a.N, at, a.N, raw);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    int64_t m = first + wave * 16 + r;
+    load(m);
+    for (; m - r + 16 <= end; m += 64) strip(m, Flag<true>{});
+    if (m - r < end) strip(m, Flag<false>{});
 }
 
 // Longer contracted dimensions, where the products count more than the bytes:
@@ -162,7 +187,7 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, KCH, NT>())) void linear_
 // (the LDS port, 128 bytes a clock, would bound RS = 1: 8 clocks a fragment
 // and wavefront, 16 clocks a matrix instruction).  The next step's operands
 // are loaded while this one's are multiplied.
-template <class T, bool Q8, int EPI, int RS, int NT>
+template <class T, bool Q8, int EPI, int RS, int NT, bool WIDE>
 __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
@@ -195,14 +220,14 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     }
 
     u32x4 wr[WL];
-    RowRaw<T, Q8> xr[RS][CH];
+    RowRaw<T, Q8, WIDE> xr[RS][CH];
     auto load = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < WL; ++i) {
             const int slot = i * 256 + tid;
             const int c = slot / (NT * 64), t = (slot / 64) % NT, l = slot & 63;
             const int n = n0 + tile_column<T>(t, l & 15);
-            wr[i] = issue_row(w + (int64_t)(n < a.N ? n : a.N - 1) * a.K, k0 + c * KC + (l >> 4) * E, a.K);
+            wr[i] = issue_row<T, WIDE>(w + (int64_t)(n < a.N ? n : a.N - 1) * a.K, k0 + c * KC + (l >> 4) * E, a.K);
         }
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -215,7 +240,7 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
             const int slot = i * 256 + tid;
             if (CH * NT % 4 != 0 && slot >= CH * NT * 64) break;
             const int c = slot / (NT * 64), t = (slot / 64) % NT, l = slot & 63;
-            const u32x4 v = finish_row<T>(wr[i], k0 + c * KC + (l >> 4) * E, a.K);
+            const u32x4 v = finish_chunk<T, WIDE>(wr[i], k0 + c * KC, k0 + c * KC + (l >> 4) * E, a.K);
             w_lds[buffer][slot] = n0 + tile_column<T>(t, l & 15) < a.N ? v : u32x4{0u, 0u, 0u, 0u};
         }
     };
@@ -234,7 +259,7 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
 #pragma unroll
         for (int s = 0; s < RS; ++s)
 #pragma unroll
-            for (int c = 0; c < CH; ++c) xc[s][c] = xr[s][c].finish(a.x, k0 + c * KC + q * E);
+            for (int c = 0; c < CH; ++c) xc[s][c] = xr[s][c].finish_in(a.x, k0 + c * KC, k0 + c * KC + q * E);
         __syncthreads();
         const bool more = k0 + CH * KC < a.K;
         if (more) load(k0 + CH * KC);
@@ -257,20 +282,19 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
         const int64_t m = first + wave * (16 * RS) + 16 * s + r;
         if (m >= a.rows) continue;
         u32x4 o[G];
-        if (EPI == 1 || other) {
+        if constexpr (EPI != 0) {
 #pragma unroll
-            for (int g = 0; g < G; ++g) o[g] = issue_row(other + m * a.ldo, n0 + g * KC + q * E, a.N);
+            for (int g = 0; g < G; ++g) o[g] = issue_row<T, WIDE>(other + m * a.ldo, n0 + g * KC + q * E, a.N);
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const int at = g * KC + q * E;  // column within the block's tile
-            if (n0 + at >= a.N) continue;
             float z[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) z[i] = acc[s][g * TG + i / 4][i & 3] + bias_lds[at + i];
             u32x4 raw = {0u, 0u, 0u, 0u};
-            if (EPI == 1 || other) raw = finish_row<T>(o[g], n0 + at, a.N);
-            store_row(y + m * a.N, n0 + at, a.N, linear_end<T, EPI, E>(a, z, raw));
+            if constexpr (EPI != 0) raw = finish_chunk<T, WIDE>(o[g], n0 + g * KC, n0 + at, a.N);
+            store_chunk(y + m * a.N, n0 + g * KC, n0 + at, a.N, linear_end<T, EPI, E>(a, z, raw));
         }
     }
 }
@@ -291,7 +315,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ w,
 }
 
 struct LinearGradW {
-    Rows x;          // channels 0: only db
+    Rows x;
     const void* dz;
     int64_t ldz;
     int64_t rows, rows_per_split;
@@ -450,7 +474,7 @@ static int chunks_of(int channels) {
     return chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : 8;
 }
 
-template <class T, bool Q8, int EPI, int KCH, int NT>
+template <class T, bool Q8, int EPI, int KCH, int NT, bool WIDE>
 static void launch_stream_as(LinearRows a, hipStream_t stream) {
     a.n_tiles = (a.N + 16 * NT - 1) / (16 * NT);
     // 512 rows a block at most, fewer where that would leave less than eight
@@ -459,36 +483,48 @@ static void launch_stream_as(LinearRows a, hipStream_t stream) {
     a.strips = (int)(strips < 4 ? 4 : strips > 32 ? 32 : strips);
     const int64_t row_blocks = (a.rows + 16 * a.strips - 1) / (16 * a.strips);
     const int64_t blocks = (row_blocks + 7) / 8 * 8 * a.n_tiles;
-    hipLaunchKernelGGL((linear_stream_kernel<T, Q8, EPI, KCH, NT>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((linear_stream_kernel<T, Q8, EPI, KCH, NT, WIDE>), dim3((unsigned)blocks), dim3(256), 0, stream,
+                       a);
 }
-template <class T, bool Q8, int EPI, int KCH>
-static void launch_stream(const LinearRows& a, hipStream_t stream) {
-    // Few rows: narrow column tiles, so that many compute units read the
-    // weights at once.
-    if (a.N <= 32 || a.rows <= 1024) launch_stream_as<T, Q8, EPI, KCH, 2>(a, stream);
-    else if (a.N <= 64) launch_stream_as<T, Q8, EPI, KCH, 4>(a, stream);
-    else launch_stream_as<T, Q8, EPI, KCH, 8>(a, stream);
-}
-
-template <class T, bool Q8, int EPI, int RS, int NT>
-static void launch_rows_as(LinearRows a, hipStream_t stream) {
+template <class T, bool Q8, int EPI, int RS, int NT, bool WIDE>
+static void launch_long_as(LinearRows a, hipStream_t stream) {
     a.n_tiles = (a.N + 16 * NT - 1) / (16 * NT);
     const int64_t row_blocks = (a.rows + 64 * RS - 1) / (64 * RS);
     const int64_t blocks = (row_blocks + 7) / 8 * 8 * a.n_tiles;
-    hipLaunchKernelGGL((linear_rows_kernel<T, Q8, EPI, RS, NT>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((linear_rows_kernel<T, Q8, EPI, RS, NT, WIDE>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
 }
 
+// Few rows: narrow column tiles, so that many compute units read the weights
+// at once.
+static bool few_rows(const LinearRows& a) { return a.rows <= 1024; }
+
+template <class T, bool Q8, int EPI, int KCH>
+static void launch_stream(const LinearRows& a, hipStream_t stream) {
+    constexpr int E = VEC<T>;
+    if (a.K < E || a.N < E) {  // rows shorter than a vector, in or out
+        if (a.N <= 32 || few_rows(a)) return launch_stream_as<T, Q8, EPI, KCH, 2, false>(a, stream);
+        if constexpr (KCH == 1) return launch_stream_as<T, Q8, EPI, 1, 8, false>(a, stream);
+    }
+    if (a.N <= 32 || few_rows(a)) launch_stream_as<T, Q8, EPI, KCH, 2, true>(a, stream);
+    else if (a.N <= 64) launch_stream_as<T, Q8, EPI, KCH, 4, true>(a, stream);
+    else launch_stream_as<T, Q8, EPI, KCH, 8, true>(a, stream);
+}
+template <class T, bool Q8, int EPI>
+static void launch_long(const LinearRows& a, hipStream_t stream) {
+    if (a.N < VEC<T>) launch_long_as<T, Q8, EPI, 1, 2, false>(a, stream);
+    else if (few_rows(a)) launch_long_as<T, Q8, EPI, 1, 2, true>(a, stream);
+    else if (a.N <= 32) launch_long_as<T, Q8, EPI, 4, 2, true>(a, stream);
+    else if (a.N <= 64) launch_long_as<T, Q8, EPI, 4, 4, true>(a, stream);
+    else launch_long_as<T, Q8, EPI, 4, 8, true>(a, stream);
+}
 template <class T, bool Q8, int EPI>
 static void launch_rows(const LinearRows& a, hipStream_t stream) {
     switch (chunks_of<T>(a.K)) {
         case 1: return launch_stream<T, Q8, EPI, 1>(a, stream);
         case 2: return launch_stream<T, Q8, EPI, 2>(a, stream);
         case 4: return launch_stream<T, Q8, EPI, 4>(a, stream);
+        default: return launch_long<T, Q8, EPI>(a, stream);
     }
-    if (a.rows <= 1024) launch_rows_as<T, Q8, EPI, 1, 2>(a, stream);
-    else if (a.N <= 32) launch_rows_as<T, Q8, EPI, 4, 2>(a, stream);
-    else if (a.N <= 64) launch_rows_as<T, Q8, EPI, 4, 4>(a, stream);
-    else launch_rows_as<T, Q8, EPI, 4, 8>(a, stream);
 }
 
 template <class T, bool Q8, int A, int B>
@@ -559,7 +595,8 @@ static int linear_fwd(const gs3d_linear_args& g, hipStream_t stream) {
     a.x = Rows{g.x, g.x_stride, {}, g.inner};
     a.w = g.weight, a.bias = g.bias, a.other = g.residual, a.ldo = g.residual_stride, a.y = g.y;
     a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
-    launch_rows<T, false, 0>(a, stream);
+    if (g.residual) launch_rows<T, false, 2>(a, stream);
+    else launch_rows<T, false, 0>(a, stream);
     return launch_status("gs3d_linear_fwd");
 }
 
@@ -567,9 +604,12 @@ template <class T, bool Q8>
 static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t stream) {
     const BwdPlan p = bwd_plan<T>(g.rows, g.inner, g.outer);
     const BwdScratch at = bwd_scratch<T>(g.rows, g.inner, g.outer);
-    // Without an activation only dW sees the input: no channels otherwise.
-    const int seen = g.grad_weight || g.activation != GS3D_ACT_NONE ? g.inner : 0;
-    const Rows x{g.x, g.x_stride, {g.codes, g.scales, seen}, seen};
+    // Without an activation only dW sees the input.  Where neither is wanted the
+    // caller may not have it: a row of the weights then stands in for every
+    // row, and the dW that comes of it is dropped.
+    const bool seen = g.grad_weight || g.activation != GS3D_ACT_NONE;
+    if (!seen && Q8) return linear_bwd<T, false>(g, scratch, stream);
+    const Rows x{seen ? g.x : g.weight, seen ? g.x_stride : 0, {g.codes, g.scales, g.inner}, g.inner};
     const bool params = g.grad_weight || g.grad_bias;
     float* part = reinterpret_cast<float*>(scratch + at.part);
     if (p.fused) {

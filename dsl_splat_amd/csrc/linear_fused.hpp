@@ -19,43 +19,60 @@ struct LinearFused {
     int K, N, act;
 };
 
-// A block of 4 wavefronts takes 64 rows at a time, KCH chunks of K and NCH of
+template <bool V>
+struct Flag {
+    static constexpr bool value = V;
+};
+
+// Wavefronts a SIMD: four where the registers do without scratch memory (128 x
+// 128 of bfloat16 at four: 681 us for the case below).
+template <class T, int KCH, int NCH>
+constexpr int fused_waves() {
+    return KCH == 8 || KCH * NCH >= (sizeof(T) == 4 ? 32 : 16) ? 2 : 4;
+}
+
+// A block of 8 wavefronts takes 64 rows at a time, KCH chunks of K and NCH of
 // N wide, over a range of rows of its own.
 //
-// A wavefront's 16 rows first: lane l holds row l % 16 and the elements from
-// VEC (l / 16) on of every chunk, of x as of dy.  With W's rows as the first
-// operand, z comes out with that row in that lane and, W's rows dealt out as
-// tile_column says, with dy's elements beside it: dz = dy act'(z) is then a
-// fragment as it stands, the second operand of dx = dz W.  W lies in LDS once,
-// row by row; dx's first operand is read from it transposed.
+// First dz.  Wavefronts s and s + 4 take rows 16 s..16 s + 15, every other
+// chunk of N each: lane l holds row l % 16 and the elements from VEC (l / 16)
+// on of a chunk, of x as of dy.  With W's rows as the first operand, z comes
+// out with that row in that lane and, W's rows dealt out as tile_column says,
+// with dy's elements beside it, so dz = dy act'(z) is whole vectors of a row.
+// dz and x go to LDS, row by row.
 //
-// dW = dz^T x contracts over rows, which are spread over lanes: dz and x go to
-// LDS row by row, and all wavefronts read them transposed, each for a quarter
-// of dW (2 x 2), which stays in its registers over all the block's rows.
+// Then dx = dz W and dW = dz^T x.  dx takes dz from LDS as it lies and W
+// transposed (W is in LDS once, row by row), every other chunk of K a
+// wavefront.  dW contracts over rows: both operands are read transposed, and
+// each wavefront's share of its tiles (4 x 2) stays in its registers over all
+// the block's rows.
 //
-// Bytes bound it where K and N are small (x and dy in, dx out): the next 64
-// rows are loaded while these are multiplied, and two blocks share a compute
-// unit where their LDS fits.
-template <class T, bool Q8, int KCH, int NCH>
-__global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a) {
+// Bytes bound it where K and N are small (x and dy in, dx out).  The next 64
+// rows are loaded as soon as these are used; two blocks, 16 wavefronts, share a
+// compute unit where their LDS fits, so one block's loads and slopes run under
+// the other's products.  With 4 wavefronts a block, each with a quarter of dW
+// and its rows' whole dz in registers, half as many fit (1600 x 1200 x 128 to
+// 128 channels of bfloat16: 426 us; float 33 to 97, three such images of 801 x
+// 601: 962 us with one wavefront a SIMD).
+template <class T, bool Q8, int KCH, int NCH, bool WIDE>
+__global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_fused_kernel(LinearFused a) {
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
-    constexpr int TG = KC / 16;              // tiles a chunk
+    constexpr int TG = KC / 16;  // tiles a chunk
     constexpr int KT = KCH * TG, NT = NCH * TG;
-    // dW's tiles over the wavefronts: 2 x 2, or for float, whose matrix
-    // instructions count most and skip what lies past K or N, N's dealt to all
-    // four (33 x 97: at most 2 x 3 tiles a wavefront, not 4 x 2).
-    constexpr int WN = sizeof(T) == 4 && NT >= 4 ? 4 : 2, WK = 4 / WN;
-    constexpr int TN = NT / WN, TK = KT / WK;
-    constexpr bool SKIP = sizeof(T) == 4;
+    constexpr int WN = 4, WK = 2;
+    constexpr int TN = (NT + WN - 1) / WN, TK = KT / WK;
+    constexpr int HN = (NCH + 1) / 2, HK = (KCH + 1) / 2;
+    constexpr bool SKIP = sizeof(T) == 4;  // matrix instructions bound float: none for what lies past K or N
     constexpr int PK = KCH * 4 + 1, PN = NCH * 4 + 1;  // pitches: the odd unit spreads rows over the banks
     __shared__ u32x4 w_lds[NCH * KC * PK];
     __shared__ u32x4 x_lds[64 * PK];
     __shared__ u32x4 z_lds[64 * PN];
-    __shared__ float bias_lds[NCH * KC];
+    __shared__ f32x4 bias_lds[NCH * KC / 4];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, q = lane >> 4;
+    const int strip = (wave & 3) * 16, half = wave >> 2;
     const int wn = wave / WK, wk = wave % WK;
     const int64_t begin = blockIdx.x * a.rows_per_block;
     const int64_t end = begin + a.rows_per_block < a.rows ? begin + a.rows_per_block : a.rows;
@@ -63,19 +80,13 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
     const T* dy = static_cast<const T*>(a.dy);
     T* dx = static_cast<T*>(a.dx);
 
-    for (int i = tid; i < NCH * KC * KCH * 4; i += 256) {
+    for (int i = tid; i < NCH * KC * KCH * 4; i += 512) {
         const int n = i / (KCH * 4), u = i % (KCH * 4);
         w_lds[n * PK + u] = n < a.N ? load_row(w + (int64_t)n * a.K, u * E, a.K) : u32x4{0u, 0u, 0u, 0u};
     }
-    for (int n = tid; n < NCH * KC; n += 256)
-        bias_lds[n] = a.bias && n < a.N ? to_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
-
-    RowRaw<T, Q8> xr[KCH];
-    u32x4 yr[NCH];
-    auto row_of = [&](int64_t m0) {  // past the end: the last row again
-        const int64_t m = m0 + wave * 16 + r;
-        return m < end ? m : end - 1;
-    };
+    for (int n = tid; n < NCH * KC; n += 512)
+        reinterpret_cast<float*>(bias_lds)[n] =
+            a.bias && n < a.N ? to_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
 
     f32x4 acc[TN][TK], acc_b[TN];
 #pragma unroll
@@ -89,43 +100,48 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
     for (int i = 0; i < E; ++i) one[i] = 1.0f;
     const u32x4 ones = pack<T>(one);
 
-    if (begin < end) {
-        const int64_t m = row_of(begin);
+    RowRaw<T, Q8, WIDE> xr[KCH];
+    u32x4 yr[HN];
+    auto row_of = [&](int64_t m0) {  // past the end: the last row again
+        const int64_t m = m0 + strip + r;
+        return m < end ? m : end - 1;
+    };
+    auto load_x = [&](int64_t m) {
 #pragma unroll
         for (int c = 0; c < KCH; ++c) xr[c].issue(a.x, m, c * KC + q * E);
+    };
+    auto load_y = [&](int64_t m, int gi) {
+        yr[gi] = issue_row<T, WIDE>(dy + m * a.ldy, (2 * gi + half) * KC + q * E, a.N);
+    };
+    if (begin < end) {
+        const int64_t m = row_of(begin);
+        load_x(m);
 #pragma unroll
-        for (int g = 0; g < NCH; ++g) yr[g] = issue_row(dy + m * a.ldy, g * KC + q * E, a.N);
+        for (int gi = 0; gi < HN; ++gi) load_y(m, gi);
     }
-    for (int64_t m0 = begin; m0 < end; m0 += 64) {
-        const int64_t m = m0 + wave * 16 + r, next = row_of(m0 + 64);
-        const bool valid = m < end;
+    __syncthreads();  // W is there
+
+    auto step = [&](int64_t m0, auto whole) {
+        const int64_t m = m0 + strip + r, next = row_of(m0 + 64);
+        const bool valid = whole.value || m < end;
+        const u32x4 zero = {0u, 0u, 0u, 0u};
         u32x4 xf[KCH];
 #pragma unroll
-        for (int c = 0; c < KCH; ++c) xf[c] = xr[c].finish(a.x, c * KC + q * E);
-        if (m0 + 64 > end) {  // rows past the end add nothing, whatever the last row holds
-#pragma unroll
-            for (int c = 0; c < KCH; ++c) xf[c] = valid ? xf[c] : u32x4{0u, 0u, 0u, 0u};
-        } else {
-#pragma unroll
-            for (int c = 0; c < KCH; ++c) xr[c].issue(a.x, next, c * KC + q * E);
+        for (int c = 0; c < KCH; ++c) {
+            xf[c] = xr[c].finish_in(a.x, c * KC, c * KC + q * E);
+            if (!valid) xf[c] = zero;  // rows past the end add nothing, whatever the last row holds
+            if (a.part && (KCH == 1 ? half == 0 : (c & 1) == half)) x_lds[(strip + r) * PK + c * 4 + q] = xf[c];
         }
-        __syncthreads();  // the tiles' last readers are done (and W is there)
-        if (a.part) {
 #pragma unroll
-            for (int c = 0; c < KCH; ++c) x_lds[(wave * 16 + r) * PK + c * 4 + q] = xf[c];
-        }
-        f32x4 out[KT];
-#pragma unroll
-        for (int t = 0; t < KT; ++t) out[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int g = 0; g < NCH; ++g) {
-            if (SKIP && g * KC >= a.N) break;
-            u32x4 dz = finish_row<T>(yr[g], g * KC + q * E, a.N);
-            yr[g] = issue_row(dy + next * a.ldy, g * KC + q * E, a.N);
+        for (int gi = 0; gi < HN; ++gi) {
+            const int g = 2 * gi + half;
+            if ((NCH == 1 && half) || (SKIP && g * KC >= a.N)) break;
+            u32x4 dz = finish_chunk<T, WIDE>(yr[gi], g * KC, g * KC + q * E, a.N);
+            if constexpr (whole.value) load_y(next, gi);
             if (a.act != GS3D_ACT_NONE) {
                 f32x4 z[TG];
 #pragma unroll
-                for (int t = 0; t < TG; ++t) z[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int t = 0; t < TG; ++t) z[t] = bias_lds[g * 4 * TG + q * TG + t];
 #pragma unroll
                 for (int c = 0; c < KCH; ++c)
 #pragma unroll
@@ -135,32 +151,40 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
                 float arg[E], grad[E];
                 unpack<T>(dz, grad);
 #pragma unroll
-                for (int i = 0; i < E; ++i) arg[i] = z[i / 4][i & 3] + bias_lds[g * KC + q * E + i];
+                for (int i = 0; i < E; ++i) arg[i] = z[i / 4][i & 3];
                 pull_back(grad, arg, a.act);
                 dz = pack<T>(grad);
             }
-            if (m0 + 64 > end) dz = valid ? dz : u32x4{0u, 0u, 0u, 0u};
-            if (a.part) z_lds[(wave * 16 + r) * PN + g * 4 + q] = dz;
-            if (dx) {
-#pragma unroll
-                for (int t = 0; t < KT; ++t) {
-                    if (SKIP && t * 16 >= a.K) break;
-                    out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, t, lane), dz, out[t],
-                                               a.N - g * KC);
-                }
-            }
+            z_lds[(strip + r) * PN + g * 4 + q] = valid ? dz : zero;
         }
-        if (dx && valid) {
+        if constexpr (whole.value) load_x(next);
+        __syncthreads();
+        if (dx) {
+            u32x4 dz[NCH];
 #pragma unroll
-            for (int c = 0; c < KCH; ++c) {
+            for (int g = 0; g < NCH; ++g) dz[g] = z_lds[(strip + r) * PN + g * 4 + q];
+#pragma unroll
+            for (int ci = 0; ci < HK; ++ci) {
+                const int c = 2 * ci + half;
+                if ((KCH == 1 && half) || (SKIP && c * KC >= a.K)) break;
+                f32x4 out[TG];
+#pragma unroll
+                for (int t = 0; t < TG; ++t) out[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int g = 0; g < NCH; ++g) {
+                    if (SKIP && g * KC >= a.N) break;
+#pragma unroll
+                    for (int t = 0; t < TG; ++t)
+                        out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, c * TG + t, lane), dz[g],
+                                                   out[t], a.N - g * KC);
+                }
                 float v[E];
 #pragma unroll
-                for (int i = 0; i < E; ++i) v[i] = out[c * TG + i / 4][i & 3];
-                store_row(dx + m * a.K, c * KC + q * E, a.K, pack<T>(v));
+                for (int i = 0; i < E; ++i) v[i] = out[i / 4][i & 3];
+                if (valid) store_chunk(dx + m * a.K, c * KC, c * KC + q * E, a.K, pack<T>(v));
             }
         }
-        if (a.part) {
-            __syncthreads();
+        if (a.part && wn < NT) {
 #pragma unroll
             for (int c = 0; c < 64 / KC; ++c) {
                 u32x4 fz[TN], fx[TK];
@@ -180,9 +204,13 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_fused_kernel(LinearFused a)
                 }
             }
         }
-    }
+        __syncthreads();  // the tiles' readers are done
+    };
+    int64_t m0 = begin;
+    for (; m0 + 64 <= end; m0 += 64) step(m0, Flag<true>{});
+    if (m0 < end) step(m0, Flag<false>{});
 
-    if (!a.part) return;
+    if (!a.part || wn >= NT) return;
     float* part = a.part + (int64_t)blockIdx.x * ((int64_t)a.N * a.K + a.N);
 #pragma unroll
     for (int i = 0; i < TN; ++i)
@@ -218,7 +246,16 @@ static bool fused_fits(int K, int N) {
 
 template <class T, bool Q8, int KCH, int NCH>
 static void launch_fused_as(const LinearFused& a, int blocks, hipStream_t stream) {
-    hipLaunchKernelGGL((linear_bwd_fused_kernel<T, Q8, KCH, NCH>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    constexpr int LEAST = sizeof(T) == 4 ? 2 : 1;
+    if constexpr (KCH == LEAST || NCH == LEAST) {
+        if (a.K < VEC<T> || a.N < VEC<T>) {  // rows shorter than a vector
+            hipLaunchKernelGGL((linear_bwd_fused_kernel<T, Q8, KCH, NCH, false>), dim3((unsigned)blocks), dim3(512), 0,
+                               stream, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((linear_bwd_fused_kernel<T, Q8, KCH, NCH, true>), dim3((unsigned)blocks), dim3(512), 0, stream,
+                       a);
 }
 template <class T, bool Q8, int KCH>
 static void launch_fused_n(const LinearFused& a, int blocks, hipStream_t stream) {
