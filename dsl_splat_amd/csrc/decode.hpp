@@ -146,22 +146,23 @@ GS3D_DEV u32x4 load_row(const T* row, int at, int count) {
     return finish_row<T>(issue_row(row, at, count), at, count);
 }
 
+// Its counterpart.  store_elements writes one by one, for an LDS row with the
+// element's alignment only; `inside`: no lane's vector reaches past the row
+// (looked at as a scalar).
+template <class T>
+GS3D_DEV void store_elements(T* row, bool inside, int at, int count, u32x4 raw) {
+    constexpr int E = VEC<T>;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (!inside && at + i >= count) continue;
+        if constexpr (E == 4) reinterpret_cast<uint32_t*>(row)[at + i] = raw[i];
+        else reinterpret_cast<uint16_t*>(row)[at + i] = (uint16_t)(raw[i / 2] >> (16 * (i & 1)));
+    }
+}
 template <class T>
 GS3D_DEV void store_row(T* row, int at, int count, u32x4 raw) {
-    if (at + VEC<T> <= count) {
-        store16(row + at, raw);
-    } else if (at < count) {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (at + i < count) reinterpret_cast<uint32_t*>(row)[at + i] = raw[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (at + i < count)
-                    reinterpret_cast<uint16_t*>(row)[at + i] = (uint16_t)(raw[i / 2] >> (16 * (i & 1)));
-        }
-    }
+    if (at + VEC<T> <= count) store16(row + at, raw);
+    else if (at < count) store_elements(row, false, at, count, raw);
 }
 
 // ---------------------------------------------------------------------------
@@ -173,13 +174,15 @@ GS3D_DEV float rcp_fast(float v) { return __builtin_amdgcn_rcpf(v); }
 
 GS3D_DEV float sigmoid(float z) { return rcp_fast(1.0f + exp2_fast(z * -1.44269504f)); }
 
-// The normal distribution's upper tail at |z|, and e^(-z^2/2) on the way:
-// Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (erfc by
-// a polynomial in 1 / (1 + p x) times e^(-x^2), x = |z| / sqrt 2, absolute
-// error 1.5e-7), with the half and the sqrt 2 folded into the constants.  17
-// issue slots (the exponential and the reciprocal are quarter rate), against
-// over 40 for the library's erf, which bounded the products' epilogues.
-GS3D_DEV float normal_tail(float z, float& bell) {
+// Half the normal distribution's weight within |z|, Phi(|z|) - 1/2, and
+// e^(-z^2/2) on the way: Abramowitz and Stegun, Handbook of Mathematical
+// Functions, 7.1.26 (erfc by a polynomial in 1 / (1 + p x) times e^(-x^2),
+// x = |z| / sqrt 2, absolute error 1.5e-7), with the half and the sqrt 2 folded
+// into the constants.  With what follows it gelu takes 11 full-rate and two
+// quarter-rate instructions, its slope 13 and two; the library's erf takes over
+// 40, and the vector units bound the products that end in a gelu (1600 x 1200
+// pixels, 32 to 128 channels, forward: 324 us with erf).
+GS3D_DEV float normal_half(float z, float& bell) {
     const float t = rcp_fast(__builtin_fmaf(__builtin_fabsf(z), 0.23164188f, 1.0f));
     bell = exp2_fast(z * z * -0.72134752f);
     float p = 0.53070271f;
@@ -187,15 +190,14 @@ GS3D_DEV float normal_tail(float z, float& bell) {
     p = __builtin_fmaf(p, t, 0.71070687f);
     p = __builtin_fmaf(p, t, -0.14224837f);
     p = __builtin_fmaf(p, t, 0.12741480f);
-    return p * t * bell;
+    return __builtin_fmaf(p * -t, bell, 0.5f);
 }
 
-// z Phi(z) = max(z, 0) - |z| tail(|z|): no difference of near values.  The
-// tail is zero long before 64; past it an infinite z would meet a zero.
+// z Phi(z) = z / 2 + |z| (Phi(|z|) - 1/2).
 GS3D_DEV float gelu(float z) {
     float bell;
-    const float tail = normal_tail(z, bell);
-    return __builtin_fmaf(-__builtin_fminf(__builtin_fabsf(z), 64.0f), tail, z < 0.0f ? 0.0f : z);
+    const float half = normal_half(z, bell);
+    return __builtin_fmaf(__builtin_fabsf(z), half, 0.5f * z);
 }
 
 template <int KIND>
@@ -215,9 +217,8 @@ GS3D_DEV float slope_as(float z) {
     }
     if constexpr (KIND == GS3D_ACT_GELU) {
         float bell;
-        const float tail = normal_tail(z, bell);
-        return __builtin_fmaf(__builtin_amdgcn_fmed3f(z, -64.0f, 64.0f) * 0.39894228f, bell,
-                              z < 0.0f ? tail : 1.0f - tail);
+        const float half = normal_half(z, bell);
+        return __builtin_fmaf(z * 0.39894228f, bell, 0.5f) + __builtin_copysignf(half, z);
     }
     if constexpr (KIND == GS3D_ACT_RELU) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
     return 1.0f;
@@ -360,8 +361,9 @@ struct RowRaw {
         raw = issue_row<T, WIDE>(static_cast<const T*>(a.x) + row * a.ldx, at, a.channels);
     }
     GS3D_DEV u32x4 finish(const Rows& a, int at) const { return finish_row<T, WIDE>(raw, at, a.channels); }
-    GS3D_DEV u32x4 finish_in(const Rows& a, int first, int at) const {
-        return finish_chunk<T, WIDE>(raw, first, at, a.channels);
+    // `inside`: no lane's vector reaches past the row (looked at as a scalar).
+    GS3D_DEV u32x4 finish_in(const Rows& a, bool inside, int at) const {
+        return inside ? raw : finish_row<T, WIDE>(raw, at, a.channels);
     }
 };
 template <class T, bool WIDE>
@@ -369,8 +371,8 @@ struct RowRaw<T, true, WIDE> {
     Q8Raw raw;
     GS3D_DEV void issue(const Rows& a, int64_t row, int at) { raw = issue_row_q8<T, WIDE>(a.q8, row, at); }
     GS3D_DEV u32x4 finish(const Rows& a, int at) const { return finish_row_q8<T, WIDE>(raw, at, a.channels); }
-    GS3D_DEV u32x4 finish_in(const Rows& a, int first, int at) const {
-        return finish_row_q8<T, WIDE>(raw, at, a.channels, first + 4 * VEC<T> <= a.channels);
+    GS3D_DEV u32x4 finish_in(const Rows& a, bool inside, int at) const {
+        return finish_row_q8<T, WIDE>(raw, at, a.channels, inside);
     }
 };
 
@@ -380,6 +382,10 @@ GS3D_DEV void store_chunk(T* row, int first, int at, int count, u32x4 raw) {
     if (first + 4 * VEC<T> <= count) store16(row + at, raw);
     else store_row(row, at, count, raw);
 }
+
+// The block's wavefront as a scalar: what hangs on it branches and addresses as
+// scalars do.
+GS3D_DEV int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // ---------------------------------------------------------------------------
 // Matrix fragments.  A fragment is 16 bytes a lane: lane l holds row l % 16
@@ -407,6 +413,21 @@ GS3D_DEV f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
             c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
         return c;
     }
+}
+
+// Results of matrix instructions are not interlocked: a read needs 8 wait
+// states after a 16-bit instruction and 11 after a float one.  The compiler
+// counts them, but over an `if` between the two it can take the longer way
+// only (seen in the listing of a strip with a residual: its last element was
+// read two states after).  settle() ends a run of matrix instructions in the
+// block that they are in, before any branch on the way to their use.
+template <int N>
+GS3D_DEV void settle(f32x4 (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));  // all of them before the wait
+    asm volatile("s_nop 11" : "+v"(v[0]));
+#pragma unroll
+    for (int i = 1; i < N; ++i) asm volatile("" : "+v"(v[i]));  // and their uses after it
 }
 
 // multiply() for a chunk of which only the first `valid` elements count (the

@@ -61,6 +61,11 @@ GS3D_DEV u32x4 linear_end(const LinearRows& a, float (&z)[E], u32x4 raw_other) {
     }
 }
 
+template <bool V>
+struct Flag {
+    static constexpr bool value = V;
+};
+
 // Wavefronts a SIMD that the stream kernel's registers leave room for.
 template <class T, bool Q8, int EPI, int KCH, int NT>
 constexpr int stream_waves() {
@@ -100,7 +105,7 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
     const int64_t first = row_block * a.strips * 16;
     if (first >= a.rows) return;
     const int64_t end = first + a.strips * 16 < a.rows ? first + a.strips * 16 : a.rows;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int r = lane & 15, q = lane >> 4;
     const T* w = static_cast<const T*>(a.w);
     const T* other = static_cast<const T*>(a.other);
@@ -119,6 +124,12 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
             a.bias && n0 + tid < a.N ? to_f32(static_cast<const T*>(a.bias)[n0 + tid]) : 0.0f;
     __syncthreads();
 
+    // Outputs leave in whole row segments, by way of LDS: as they come, an
+    // instruction would write 64 bytes of 16 rows (1920 x 1080 pixels, 64 to
+    // 512 channels of float16: 754 against 508 us).  Rows that are not whole
+    // vectors leave as they come: their segments start anywhere (three images
+    // of 801 x 601, 33 to 97 channels of float: 235 against 283 us).
+    const bool staged = a.N % E == 0;
     RowRaw<T, Q8, WIDE> xr[KCH];
     auto load = [&](int64_t m) {
         m = m < end ? m : end - 1;  // rows past the end repeat the last one and are not stored
@@ -128,7 +139,7 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
     auto strip = [&](int64_t m, auto whole) {
         u32x4 xf[KCH], o[G];
 #pragma unroll
-        for (int c = 0; c < KCH; ++c) xf[c] = xr[c].finish_in(a.x, c * KC, c * KC + q * E);
+        for (int c = 0; c < KCH; ++c) xf[c] = xr[c].finish_in(a.x, c * KC + KC <= a.K, c * KC + q * E);
         if constexpr (EPI != 0) {
             const T* row = other + (whole.value || m < end ? m : end - 1) * a.ldo;
 #pragma unroll
@@ -150,16 +161,18 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
 #pragma unroll
                 for (int t = 0; t < TG; ++t)
                     acc[t] = multiply_chunk<T>(w_lds[(c * NT + g * TG + t) * 64 + mine], xf[c], acc[t], a.K - c * KC);
+            settle(acc);
             const int at = n0 + g * KC;
             float z[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) z[i] = acc[i / 4][i & 3];
             u32x4 raw = {0u, 0u, 0u, 0u};
             if constexpr (EPI != 0) raw = finish_chunk<T, WIDE>(o[g], at, at + q * E, a.N);
-            out_lds[wave][r * PO + g * 4 + q] = linear_end<T, EPI, E>(a, z, raw);
+            raw = linear_end<T, EPI, E>(a, z, raw);
+            if (staged) out_lds[wave][r * PO + g * 4 + q] = raw;
+            else if (whole.value || m < end) store_chunk(y + m * a.N, at, at + q * E, a.N, raw);
         }
-        // The strip's outputs leave in whole row segments: as they come, an
-        // instruction would write 64 bytes of 16 rows.
+        if (!staged) return;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         const int vec = lane % VP, at = n0 + vec * E;
@@ -204,7 +217,7 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     const int n0 = n_tile * 16 * NT;
     const int64_t first = row_block * (64 * RS);
     if (first >= a.rows) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int r = lane & 15, q = lane >> 4;
     const T* w = static_cast<const T*>(a.w);
 
@@ -259,7 +272,7 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
 #pragma unroll
         for (int s = 0; s < RS; ++s)
 #pragma unroll
-            for (int c = 0; c < CH; ++c) xc[s][c] = xr[s][c].finish_in(a.x, k0 + c * KC, k0 + c * KC + q * E);
+            for (int c = 0; c < CH; ++c) xc[s][c] = xr[s][c].finish_in(a.x, k0 + c * KC + KC <= a.K, k0 + c * KC + q * E);
         __syncthreads();
         const bool more = k0 + CH * KC < a.K;
         if (more) load(k0 + CH * KC);
@@ -275,6 +288,8 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
         if (more) store(k0 + CH * KC, buffer);
     }
 
+#pragma unroll
+    for (int s = 0; s < RS; ++s) settle(acc[s]);
     T* y = static_cast<T*>(a.y);
     const T* other = static_cast<const T*>(a.other);
 #pragma unroll
@@ -334,7 +349,8 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
     constexpr int KC = CHUNK<T>;
     constexpr int MR = 2 * KC;                       // rows a step
     constexpr int CZ = 32 * A / E, CX = 32 * B / E;  // vectors across dz's and x's tile
-    constexpr int PZ = CZ + 1, PX = CX + 1;          // pitches: the odd unit spreads rows over the banks
+    constexpr int PAD = sizeof(T) == 4 ? 1 : 2;      // spreads rows over the banks
+    constexpr int PZ = CZ + PAD, PX = CX + PAD;
     constexpr int LZ = (MR * CZ + 255) / 256, LX = (MR * CX + 255) / 256;
     __shared__ u32x4 z_lds[MR * PZ];
     __shared__ u32x4 x_lds[MR * PX];
@@ -347,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
     const int n0 = nt * 32 * A, k0 = kt * 32 * B;
     const int64_t begin = split * a.rows_per_split;
     const int64_t end = begin + a.rows_per_split < a.rows ? begin + a.rows_per_split : a.rows;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int r = lane & 15, q = lane >> 4;
     const int wn = wave >> 1, wk = wave & 1;
     const bool sum_bias = kt == 0 && wk == 0;
@@ -422,6 +438,9 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
         }
     }
 
+#pragma unroll
+    for (int i = 0; i < A; ++i) settle(acc[i]);
+    settle(acc_b);
     float* part = a.part + split * ((int64_t)a.N * a.K + a.N);
 #pragma unroll
     for (int i = 0; i < A; ++i)

@@ -19,27 +19,27 @@ struct LinearFused {
     int K, N, act;
 };
 
-template <bool V>
-struct Flag {
-    static constexpr bool value = V;
-};
-
 // Wavefronts a SIMD: four where the registers do without scratch memory (128 x
 // 128 of bfloat16 at four: 681 us for the case below).
 template <class T, int KCH, int NCH>
 constexpr int fused_waves() {
-    return KCH == 8 || KCH * NCH >= (sizeof(T) == 4 ? 32 : 16) ? 2 : 4;
+    // Two blocks of float fit where W and both tiles take 80 KB at most.
+    if (sizeof(T) == 4) return (NCH * 16 * (KCH * 4 + 1) + 64 * (KCH + NCH) * 4 + 128) * 16 + NCH * 64 > 81920 ? 2 : 4;
+    return 4;
 }
 
 // A block of 8 wavefronts takes 64 rows at a time, KCH chunks of K and NCH of
 // N wide, over a range of rows of its own.
 //
+// x and dy go to LDS as they lie in memory, row by row (whole lines an
+// instruction), the next 64 rows on their way while these are worked on.
+//
 // First dz.  Wavefronts s and s + 4 take rows 16 s..16 s + 15, every other
-// chunk of N each: lane l holds row l % 16 and the elements from VEC (l / 16)
-// on of a chunk, of x as of dy.  With W's rows as the first operand, z comes
-// out with that row in that lane and, W's rows dealt out as tile_column says,
-// with dy's elements beside it, so dz = dy act'(z) is whole vectors of a row.
-// dz and x go to LDS, row by row.
+// chunk of N each: lane l has row l % 16 and the elements from VEC (l / 16) on
+// of a chunk, of x as of dy.  With W's rows as the first operand, z comes out
+// with that row in that lane and, W's rows dealt out as tile_column says, with
+// dy's elements beside it, so dz = dy act'(z) takes dy's place vector by
+// vector.
 //
 // Then dx = dz W and dW = dz^T x.  dx takes dz from LDS as it lies and W
 // transposed (W is in LDS once, row by row), every other chunk of K a
@@ -47,13 +47,9 @@ constexpr int fused_waves() {
 // each wavefront's share of its tiles (4 x 2) stays in its registers over all
 // the block's rows.
 //
-// Bytes bound it where K and N are small (x and dy in, dx out).  The next 64
-// rows are loaded as soon as these are used; two blocks, 16 wavefronts, share a
-// compute unit where their LDS fits, so one block's loads and slopes run under
-// the other's products.  With 4 wavefronts a block, each with a quarter of dW
-// and its rows' whole dz in registers, half as many fit (1600 x 1200 x 128 to
-// 128 channels of bfloat16: 426 us; float 33 to 97, three such images of 801 x
-// 601: 962 us with one wavefront a SIMD).
+// Bytes bound it where K and N are small (x and dy in, dx out).  Two blocks,
+// 16 wavefronts, share a compute unit where their LDS and registers fit, so
+// one block's loads and slopes run under the other's products.
 template <class T, bool Q8, int KCH, int NCH, bool WIDE>
 __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_fused_kernel(LinearFused a) {
     constexpr int E = VEC<T>;
@@ -61,27 +57,36 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
     constexpr int TG = KC / 16;  // tiles a chunk
     constexpr int KT = KCH * TG, NT = NCH * TG;
     constexpr int WN = 4, WK = 2;
-    constexpr int TN = (NT + WN - 1) / WN, TK = KT / WK;
+    constexpr int TN = (NT + WN - 1) / WN, TK = (KT + WK - 1) / WK;
     constexpr int HN = (NCH + 1) / 2, HK = (KCH + 1) / 2;
     constexpr bool SKIP = sizeof(T) == 4;  // matrix instructions bound float: none for what lies past K or N
-    constexpr int PK = KCH * 4 + 1, PN = NCH * 4 + 1;  // pitches: the odd unit spreads rows over the banks
+    constexpr int VK = KCH * 4, VN = NCH * 4;          // vectors of a row
+    constexpr int PAD = sizeof(T) == 4 ? 1 : 2;  // spreads rows over the banks, for whole as for transposed reads
+    constexpr int PK = VK + PAD, PN = VN + PAD;
+    // Vectors are dealt to threads by powers of two a row; a row of 6 or 7
+    // chunks leaves some without.
+    constexpr int DN = NCH > 4 ? 32 : VN;
+    constexpr int LK = (64 * VK + 511) / 512, LN = (64 * DN + 511) / 512;
     __shared__ u32x4 w_lds[NCH * KC * PK];
     __shared__ u32x4 x_lds[64 * PK];
     __shared__ u32x4 z_lds[64 * PN];
     __shared__ f32x4 bias_lds[NCH * KC / 4];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int r = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, wave = wave_id();
     const int strip = (wave & 3) * 16, half = wave >> 2;
     const int wn = wave / WK, wk = wave % WK;
+    // dW's tiles that there are; for 16-bit types all of the block's, known at
+    // compile time unless they do not share out evenly.
+    const int tiles_n = SKIP ? (a.N + 15) / 16 : NT % WN ? NT : 1 << 30;
+    const int tiles_k = SKIP ? (a.K + 15) / 16 : KT % WK ? KT : 1 << 30;
     const int64_t begin = blockIdx.x * a.rows_per_block;
     const int64_t end = begin + a.rows_per_block < a.rows ? begin + a.rows_per_block : a.rows;
     const T* w = static_cast<const T*>(a.w);
     const T* dy = static_cast<const T*>(a.dy);
     T* dx = static_cast<T*>(a.dx);
 
-    for (int i = tid; i < NCH * KC * KCH * 4; i += 512) {
-        const int n = i / (KCH * 4), u = i % (KCH * 4);
+    for (int i = tid; i < NCH * KC * VK; i += 512) {
+        const int n = i / VK, u = i % VK;
         w_lds[n * PK + u] = n < a.N ? load_row(w + (int64_t)n * a.K, u * E, a.K) : u32x4{0u, 0u, 0u, 0u};
     }
     for (int n = tid; n < NCH * KC; n += 512)
@@ -100,45 +105,61 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
     for (int i = 0; i < E; ++i) one[i] = 1.0f;
     const u32x4 ones = pack<T>(one);
 
-    RowRaw<T, Q8, WIDE> xr[KCH];
-    u32x4 yr[HN];
-    auto row_of = [&](int64_t m0) {  // past the end: the last row again
-        const int64_t m = m0 + strip + r;
-        return m < end ? m : end - 1;
-    };
-    auto load_x = [&](int64_t m) {
+    RowRaw<T, Q8, WIDE> xr[LK];
+    u32x4 yr[LN];
+    auto load = [&](int64_t m0) {  // rows past the end: the last row again
 #pragma unroll
-        for (int c = 0; c < KCH; ++c) xr[c].issue(a.x, m, c * KC + q * E);
-    };
-    auto load_y = [&](int64_t m, int gi) {
-        yr[gi] = issue_row<T, WIDE>(dy + m * a.ldy, (2 * gi + half) * KC + q * E, a.N);
-    };
-    if (begin < end) {
-        const int64_t m = row_of(begin);
-        load_x(m);
-#pragma unroll
-        for (int gi = 0; gi < HN; ++gi) load_y(m, gi);
-    }
-    __syncthreads();  // W is there
-
-    auto step = [&](int64_t m0, auto whole) {
-        const int64_t m = m0 + strip + r, next = row_of(m0 + 64);
-        const bool valid = whole.value || m < end;
-        const u32x4 zero = {0u, 0u, 0u, 0u};
-        u32x4 xf[KCH];
-#pragma unroll
-        for (int c = 0; c < KCH; ++c) {
-            xf[c] = xr[c].finish_in(a.x, c * KC, c * KC + q * E);
-            if (!valid) xf[c] = zero;  // rows past the end add nothing, whatever the last row holds
-            if (a.part && (KCH == 1 ? half == 0 : (c & 1) == half)) x_lds[(strip + r) * PK + c * 4 + q] = xf[c];
+        for (int i = 0; i < LK; ++i) {
+            const int u = i * 512 + tid;
+            const int64_t m = m0 + u / VK < end ? m0 + u / VK : end - 1;
+            xr[i].issue(a.x, m, u % VK * E);
         }
 #pragma unroll
-        for (int gi = 0; gi < HN; ++gi) {
-            const int g = 2 * gi + half;
-            if ((NCH == 1 && half) || (SKIP && g * KC >= a.N)) break;
-            u32x4 dz = finish_chunk<T, WIDE>(yr[gi], g * KC, g * KC + q * E, a.N);
-            if constexpr (whole.value) load_y(next, gi);
-            if (a.act != GS3D_ACT_NONE) {
+        for (int i = 0; i < LN; ++i) {
+            const int u = i * 512 + tid;
+            const int64_t m = m0 + u / DN < end ? m0 + u / DN : end - 1;
+            yr[i] = issue_row<T, WIDE>(dy + m * a.ldy, u % DN * E, a.N);
+        }
+    };
+    // Rows past the end add nothing, whatever the last row holds.
+    auto fill = [&](int64_t m0) {
+        const u32x4 zero = {0u, 0u, 0u, 0u};
+        const bool whole = m0 + 64 <= end;
+#pragma unroll
+        for (int i = 0; i < LK; ++i) {
+            const int u = i * 512 + tid;
+            if (64 * VK % 512 != 0 && u >= 64 * VK) break;
+            u32x4 v = xr[i].finish_in(a.x, VK * E <= a.K, u % VK * E);
+            x_lds[u / VK * PK + u % VK] = whole || m0 + u / VK < end ? v : zero;
+        }
+#pragma unroll
+        for (int i = 0; i < LN; ++i) {
+            const int u = i * 512 + tid;
+            if (64 * DN % 512 != 0 && u >= 64 * DN) break;
+            u32x4 v = yr[i];
+            if (VN * E > a.N) v = finish_row<T, WIDE>(v, u % DN * E, a.N);
+            if (DN == VN || u % DN < VN) z_lds[u / DN * PN + u % DN] = whole || m0 + u / DN < end ? v : zero;
+        }
+    };
+
+    if (begin < end) load(begin);
+    for (int64_t m0 = begin; m0 < end; m0 += 64) {
+        fill(m0);
+        if (m0 + 64 < end) load(m0 + 64);
+        __syncthreads();
+        // Opaque in every round: the tiles' addresses, all of them loop
+        // invariant, would otherwise fill the registers.
+        int lane = tid & 63;
+        asm volatile("" : "+v"(lane));
+        const int r = lane & 15, q = lane >> 4;
+        if (a.act != GS3D_ACT_NONE) {
+            u32x4 xf[KCH];
+#pragma unroll
+            for (int c = 0; c < KCH; ++c) xf[c] = x_lds[(strip + r) * PK + c * 4 + q];
+#pragma unroll
+            for (int gi = 0; gi < HN; ++gi) {
+                const int g = 2 * gi + half;
+                if (g >= NCH || (SKIP && g * KC >= a.N)) break;
                 f32x4 z[TG];
 #pragma unroll
                 for (int t = 0; t < TG; ++t) z[t] = bias_lds[g * 4 * TG + q * TG + t];
@@ -148,56 +169,64 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
                     for (int t = 0; t < TG; ++t)
                         z[t] = multiply_chunk<T>(w_lds[tile_column<T>(g * TG + t, r) * PK + c * 4 + q], xf[c], z[t],
                                                  a.K - c * KC);
+                settle(z);
+                u32x4& slot = z_lds[(strip + r) * PN + g * 4 + q];
                 float arg[E], grad[E];
-                unpack<T>(dz, grad);
+                unpack<T>(slot, grad);
 #pragma unroll
                 for (int i = 0; i < E; ++i) arg[i] = z[i / 4][i & 3];
                 pull_back(grad, arg, a.act);
-                dz = pack<T>(grad);
+                slot = pack<T>(grad);
             }
-            z_lds[(strip + r) * PN + g * 4 + q] = valid ? dz : zero;
+            __syncthreads();
         }
-        if constexpr (whole.value) load_x(next);
-        __syncthreads();
         if (dx) {
-            u32x4 dz[NCH];
+            const int64_t m = m0 + strip + r;
+            // Float's twice as many vectors are read where they are used.
+            u32x4 dz[SKIP ? 1 : NCH];
+            if constexpr (!SKIP) {
 #pragma unroll
-            for (int g = 0; g < NCH; ++g) dz[g] = z_lds[(strip + r) * PN + g * 4 + q];
+                for (int g = 0; g < NCH; ++g) dz[g] = z_lds[(strip + r) * PN + g * 4 + q];
+            }
 #pragma unroll
             for (int ci = 0; ci < HK; ++ci) {
                 const int c = 2 * ci + half;
-                if ((KCH == 1 && half) || (SKIP && c * KC >= a.K)) break;
+                if (c >= KCH || (SKIP && c * KC >= a.K)) break;
                 f32x4 out[TG];
 #pragma unroll
                 for (int t = 0; t < TG; ++t) out[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int g = 0; g < NCH; ++g) {
                     if (SKIP && g * KC >= a.N) break;
+                    if constexpr (SKIP) dz[0] = z_lds[(strip + r) * PN + g * 4 + q];
 #pragma unroll
                     for (int t = 0; t < TG; ++t)
-                        out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, c * TG + t, lane), dz[g],
-                                                   out[t], a.N - g * KC);
+                        out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, c * TG + t, lane),
+                                                   dz[SKIP ? 0 : g], out[t], a.N - g * KC);
                 }
+                settle(out);
                 float v[E];
 #pragma unroll
                 for (int i = 0; i < E; ++i) v[i] = out[i / 4][i & 3];
-                if (valid) store_chunk(dx + m * a.K, c * KC, c * KC + q * E, a.K, pack<T>(v));
+                if (m < end) store_chunk(dx + m * a.K, c * KC, c * KC + q * E, a.K, pack<T>(v));
             }
         }
-        if (a.part && wn < NT) {
+        if (a.part) {
 #pragma unroll
             for (int c = 0; c < 64 / KC; ++c) {
                 u32x4 fz[TN], fx[TK];
 #pragma unroll
-                for (int i = 0; i < TN; ++i) fz[i] = read_transposed<T, false>(z_lds, PN, c * KC, i * WN + wn, lane);
+                for (int i = 0; i < TN; ++i)
+                    if (i * WN + wn < tiles_n) fz[i] = read_transposed<T, false>(z_lds, PN, c * KC, i * WN + wn, lane);
 #pragma unroll
-                for (int j = 0; j < TK; ++j) fx[j] = read_transposed<T, false>(x_lds, PK, c * KC, j * WK + wk, lane);
+                for (int j = 0; j < TK; ++j)
+                    if (j * WK + wk < tiles_k) fx[j] = read_transposed<T, false>(x_lds, PK, c * KC, j * WK + wk, lane);
 #pragma unroll
                 for (int i = 0; i < TN; ++i) {
-                    if (SKIP && (i * WN + wn) * 16 >= a.N) break;
+                    if (i * WN + wn >= tiles_n) break;
 #pragma unroll
                     for (int j = 0; j < TK; ++j) {
-                        if (SKIP && (j * WK + wk) * 16 >= a.K) break;
+                        if (j * WK + wk >= tiles_k) break;
                         acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
                     }
                     if (wk == 0) acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
@@ -205,12 +234,13 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
             }
         }
         __syncthreads();  // the tiles' readers are done
-    };
-    int64_t m0 = begin;
-    for (; m0 + 64 <= end; m0 += 64) step(m0, Flag<true>{});
-    if (m0 < end) step(m0, Flag<false>{});
+    }
 
-    if (!a.part || wn >= NT) return;
+    if (!a.part) return;
+    const int r = tid & 15, q = (tid & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) settle(acc[i]);
+    settle(acc_b);
     float* part = a.part + (int64_t)blockIdx.x * ((int64_t)a.N * a.K + a.N);
 #pragma unroll
     for (int i = 0; i < TN; ++i)
@@ -227,21 +257,27 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
         }
 }
 
-// Widths are covered by 1, 2, 4 or 8 chunks (float: 2, 4 or 8, so that dW's
-// tiles split over 2 x 2 wavefronts), as far as a wavefront's quarter of dW
-// stays in 64 registers: 128 x 128, 64 x 256, 32 x 256 of 16-bit types and
-// 128 x 128 of float.
+// Widths of 16-bit types are covered by 1, 2, 4 or 8 chunks, as far as a
+// wavefront's share of dW stays in 32 registers: 128 x 128, 64 x 256, 256 x 64.
+// Float's chunks are half as wide, 2, 4 or 8 of K, 2, 4, 6, 7 or 8 of N: LDS
+// decides how many blocks share a compute unit (33 to 97: 78 KB at 4 x 7, two
+// blocks; 87 KB at 4 x 8, one).
 template <class T>
-static int fused_chunks(int channels) {
-    const int least = sizeof(T) == 4 ? 2 : 1;
-    int chunks = 8;
-    while (chunks > least && channels <= chunks / 2 * CHUNK<T>) chunks /= 2;
-    return chunks;
+static int fused_chunks_k(int channels) {
+    const int chunks = (channels + CHUNK<T> - 1) / CHUNK<T>;
+    if (sizeof(T) == 4) return chunks <= 2 ? 2 : chunks <= 4 ? 4 : 8;
+    return chunks <= 2 ? chunks : chunks <= 4 ? 4 : 8;
+}
+template <class T>
+static int fused_chunks_n(int channels) {
+    const int chunks = (channels + CHUNK<T> - 1) / CHUNK<T>;
+    if (sizeof(T) == 4) return chunks <= 2 ? 2 : chunks <= 4 ? 4 : chunks <= 6 ? 6 : chunks;
+    return chunks <= 2 ? chunks : chunks <= 4 ? 4 : 8;
 }
 template <class T>
 static bool fused_fits(int K, int N) {
     if (K > 8 * CHUNK<T> || N > 8 * CHUNK<T>) return false;
-    return sizeof(T) == 4 || fused_chunks<T>(K) * fused_chunks<T>(N) <= 16;
+    return sizeof(T) == 4 || fused_chunks_k<T>(K) * fused_chunks_n<T>(N) <= 16;
 }
 
 template <class T, bool Q8, int KCH, int NCH>
@@ -259,29 +295,36 @@ static void launch_fused_as(const LinearFused& a, int blocks, hipStream_t stream
 }
 template <class T, bool Q8, int KCH>
 static void launch_fused_n(const LinearFused& a, int blocks, hipStream_t stream) {
-    constexpr int MOST = sizeof(T) == 4 ? 64 : 16;
-    switch (fused_chunks<T>(a.N)) {
+    constexpr bool F = sizeof(T) == 4;
+    switch (fused_chunks_n<T>(a.N)) {
         case 1:
-            if constexpr (sizeof(T) == 2) launch_fused_as<T, Q8, KCH, 1>(a, blocks, stream);
+            if constexpr (!F) launch_fused_as<T, Q8, KCH, 1>(a, blocks, stream);
             break;
         case 2: launch_fused_as<T, Q8, KCH, 2>(a, blocks, stream); break;
         case 4:
-            if constexpr (KCH * 4 <= MOST) launch_fused_as<T, Q8, KCH, 4>(a, blocks, stream);
+            if constexpr (F || KCH <= 4) launch_fused_as<T, Q8, KCH, 4>(a, blocks, stream);
             break;
-        default:
-            if constexpr (KCH * 8 <= MOST) launch_fused_as<T, Q8, KCH, 8>(a, blocks, stream);
+        case 6:
+            if constexpr (F) launch_fused_as<T, Q8, KCH, 6>(a, blocks, stream);
+            break;
+        case 7:
+            if constexpr (F) launch_fused_as<T, Q8, KCH, 7>(a, blocks, stream);
+            break;
+        case 8:
+            if constexpr (F || KCH <= 2) launch_fused_as<T, Q8, KCH, 8>(a, blocks, stream);
             break;
     }
 }
 template <class T, bool Q8>
 static void launch_fused(const LinearFused& a, int blocks, hipStream_t stream) {
-    switch (fused_chunks<T>(a.K)) {
+    constexpr bool F = sizeof(T) == 4;
+    switch (fused_chunks_k<T>(a.K)) {
         case 1:
-            if constexpr (sizeof(T) == 2) launch_fused_n<T, Q8, 1>(a, blocks, stream);
+            if constexpr (!F) launch_fused_n<T, Q8, 1>(a, blocks, stream);
             break;
         case 2: launch_fused_n<T, Q8, 2>(a, blocks, stream); break;
         case 4: launch_fused_n<T, Q8, 4>(a, blocks, stream); break;
-        default: launch_fused_n<T, Q8, 8>(a, blocks, stream); break;
+        case 8: launch_fused_n<T, Q8, 8>(a, blocks, stream); break;
     }
 }
 
