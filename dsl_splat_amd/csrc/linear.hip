@@ -4,9 +4,12 @@
 namespace gs3d {
 
 // Defined by linear_f32.hip, linear_bf16.hip, linear_f16.hip.
-int linear_fwd_f32(const gs3d_linear_args& g, hipStream_t stream);
-int linear_fwd_bf16(const gs3d_linear_args& g, hipStream_t stream);
-int linear_fwd_f16(const gs3d_linear_args& g, hipStream_t stream);
+size_t linear_fwd_bytes_f32(int64_t rows, int K, int N);
+int linear_fwd_f32(const gs3d_linear_args& g, void* scratch, hipStream_t stream);
+size_t linear_fwd_bytes_bf16(int64_t rows, int K, int N);
+int linear_fwd_bf16(const gs3d_linear_args& g, void* scratch, hipStream_t stream);
+size_t linear_fwd_bytes_f16(int64_t rows, int K, int N);
+int linear_fwd_f16(const gs3d_linear_args& g, void* scratch, hipStream_t stream);
 int linear_bwd_f32(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t stream);
 int linear_bwd_bf16(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t stream);
 int linear_bwd_f16(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t stream);
@@ -21,14 +24,23 @@ static bool linear_sizes_ok(int64_t rows, int K, int N, int dtype, int activatio
 
 }  // namespace gs3d
 
-extern "C" int gs3d_linear_fwd(const gs3d_linear_args* g, void* stream) {
+extern "C" size_t gs3d_linear_fwd_scratch_bytes(int64_t rows, int32_t inner, int32_t outer, int32_t dtype) {
+    if (!gs3d::linear_sizes_ok(rows, inner, outer, dtype, 0)) return 0;
+    if (dtype == GS3D_F32) return gs3d::linear_fwd_bytes_f32(rows, inner, outer);
+    return dtype == GS3D_BF16 ? gs3d::linear_fwd_bytes_bf16(rows, inner, outer)
+                              : gs3d::linear_fwd_bytes_f16(rows, inner, outer);
+}
+
+extern "C" int gs3d_linear_fwd(const gs3d_linear_args* g, void* scratch, size_t scratch_bytes, void* stream) {
     if (!g || !gs3d::linear_sizes_ok(g->rows, g->inner, g->outer, g->dtype, g->activation)) return GS3D_ERR_ARGUMENT;
     if (g->x_stride < g->inner || (g->residual && g->residual_stride < g->outer)) return GS3D_ERR_ARGUMENT;
     if (g->rows == 0) return GS3D_OK;
     if (!g->x || !g->weight || !g->y) return GS3D_ERR_ARGUMENT;
+    const size_t needed = gs3d_linear_fwd_scratch_bytes(g->rows, g->inner, g->outer, g->dtype);
+    if (needed > 0 && (!scratch || scratch_bytes < needed)) return GS3D_ERR_SCRATCH;
     const hipStream_t s = gs3d::as_stream(stream);
-    if (g->dtype == GS3D_F32) return gs3d::linear_fwd_f32(*g, s);
-    return g->dtype == GS3D_BF16 ? gs3d::linear_fwd_bf16(*g, s) : gs3d::linear_fwd_f16(*g, s);
+    if (g->dtype == GS3D_F32) return gs3d::linear_fwd_f32(*g, scratch, s);
+    return g->dtype == GS3D_BF16 ? gs3d::linear_fwd_bf16(*g, scratch, s) : gs3d::linear_fwd_f16(*g, scratch, s);
 }
 
 extern "C" size_t gs3d_linear_bwd_scratch_bytes(int64_t rows, int32_t inner, int32_t outer, int32_t dtype) {

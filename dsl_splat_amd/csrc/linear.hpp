@@ -66,6 +66,31 @@ struct Flag {
     static constexpr bool value = V;
 };
 
+// Orders a wavefront's own LDS accesses (the LDS takes them in order; this is
+// for the compiler).
+GS3D_DEV void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wavefront's strip of 16 rows x VP vectors, in LDS at pitch PO, to rows from
+// `first` on and columns from n0 on, whole row segments an instruction.
+template <class T, int VP, int PO, class Whole>
+GS3D_DEV void store_strip(const u32x4* strip, T* y, int64_t first, int64_t end, int n0, int N, int lane, Whole) {
+    constexpr int E = VEC<T>;
+    wave_fence();
+    const int vec = lane % VP, at = n0 + vec * E;
+#pragma unroll
+    for (int i = 0; i < 16 * VP / 64; ++i) {
+        const int row = i * (64 / VP) + lane / VP;
+        const u32x4 raw = strip[row * PO + vec];
+        const int64_t to = first + row;
+        if (Whole::value && n0 + VP * E <= N) store16(y + to * N + at, raw);
+        else if (to < end) store_row(y + to * N, at, N, raw);
+    }
+    wave_fence();
+}
+
 // Wavefronts a SIMD that the stream kernel's registers leave room for.
 template <class T, bool Q8, int EPI, int KCH, int NT>
 constexpr int stream_waves() {
@@ -76,12 +101,17 @@ constexpr int stream_waves() {
 
 // A block of 4 wavefronts holds the weights of 16 NT columns in LDS, in
 // fragment order (one 1 KB run per chunk and tile, read without conflicts),
-// and takes strips of 16 rows from a range of a.strips of them.  A wavefront
-// reads its strip straight into fragments, 64 bytes of a row at a time, the
-// next strip while this one is multiplied; the wavefronts never wait for one
-// another.  W's rows are the first operand, so a lane ends with 16 bytes of
-// one output row; the sums start at the bias.  HBM bounds it while K and N are
-// small.
+// and takes strips of 16 rows from a range of a.strips of them; the
+// wavefronts never wait for one another.  W's rows are the first operand, so
+// a lane ends with 16 bytes of one output row; the sums start at the bias.
+// HBM bounds it while K and N are small.
+//
+// A fragment has one row in every lane of 16, and the memory pipeline joins
+// neighbouring lanes only: read as fragments, 1 KB takes 64 accesses of 16
+// bytes.  So a strip's rows, of x, of dy or the residual and of y, move in
+// whole row segments, neighbouring lanes on neighbouring vectors, and change
+// their layout in LDS that is the wavefront's own (1920 x 1080 pixels, 64 to
+// 512 channels of float16: 754 us with fragments written as they come).
 //
 // Loads wait for the stores issued before them, so the next strip's are issued
 // first, and whole strips store without a branch: the wait for a load then
@@ -92,10 +122,12 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
     constexpr int KC = CHUNK<T>;
     constexpr int TG = KC / 16;  // tiles of a lane's 16-byte output vector
     constexpr int G = NT / TG;
-    constexpr int VP = 16 * NT / E;  // vectors of a full output row
-    constexpr int PO = VP + 1;       // pitch of an output row in LDS
+    constexpr int PAD = sizeof(T) == 4 ? 1 : 2;
+    constexpr int VK = KCH * 4, PK = VK + PAD;      // an input row's vectors, and its pitch in LDS
+    constexpr int VP = 16 * NT / E, PO = VP + PAD;  // an output row's
+    constexpr int LK = 16 * VK / 64, LP = 16 * VP / 64;
     __shared__ u32x4 w_lds[KCH * NT * 64];
-    __shared__ u32x4 out_lds[4][16 * PO];
+    __shared__ u32x4 strip_lds[4][16 * (PK > PO ? PK : PO)];
     __shared__ f32x4 bias_lds[4 * NT];
 
     int64_t row_block;
@@ -110,6 +142,18 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
     const T* w = static_cast<const T*>(a.w);
     const T* other = static_cast<const T*>(a.other);
     T* y = static_cast<T*>(a.y);
+    u32x4* mine = strip_lds[wave];
+
+    RowRaw<T, Q8, WIDE> xr[LK];
+    auto load = [&](int64_t m0) {  // rows past the end repeat the last one and are not stored
+#pragma unroll
+        for (int i = 0; i < LK; ++i) {
+            const int64_t m = m0 + i * (64 / VK) + lane / VK;
+            xr[i].issue(a.x, m < end ? m : end - 1, lane % VK * E);
+        }
+    };
+    int64_t m0 = first + wave * 16;
+    load(m0);
 
 #pragma unroll
     for (int i = 0; i < (KCH * NT + 3) / 4; ++i) {
@@ -124,73 +168,67 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
             a.bias && n0 + tid < a.N ? to_f32(static_cast<const T*>(a.bias)[n0 + tid]) : 0.0f;
     __syncthreads();
 
-    // Outputs leave in whole row segments, by way of LDS: as they come, an
-    // instruction would write 64 bytes of 16 rows (1920 x 1080 pixels, 64 to
-    // 512 channels of float16: 754 against 508 us).  Rows that are not whole
-    // vectors leave as they come: their segments start anywhere (three images
-    // of 801 x 601, 33 to 97 channels of float: 235 against 283 us).
-    const bool staged = a.N % E == 0;
-    RowRaw<T, Q8, WIDE> xr[KCH];
-    auto load = [&](int64_t m) {
-        m = m < end ? m : end - 1;  // rows past the end repeat the last one and are not stored
+    const bool staged = a.N % E == 0;  // else segments start anywhere, and vectors leave as they come
+    auto strip = [&](int64_t m0, auto whole) {
+        u32x4 xf[KCH];
 #pragma unroll
-        for (int c = 0; c < KCH; ++c) xr[c].issue(a.x, m, c * KC + q * E);
-    };
-    auto strip = [&](int64_t m, auto whole) {
-        u32x4 xf[KCH], o[G];
-#pragma unroll
-        for (int c = 0; c < KCH; ++c) xf[c] = xr[c].finish_in(a.x, c * KC + KC <= a.K, c * KC + q * E);
+        for (int i = 0; i < LK; ++i)
+            mine[(i * (64 / VK) + lane / VK) * PK + lane % VK] = xr[i].finish_in(a.x, VK * E <= a.K, lane % VK * E);
+        u32x4 o[LP];
         if constexpr (EPI != 0) {
-            const T* row = other + (whole.value || m < end ? m : end - 1) * a.ldo;
 #pragma unroll
-            for (int g = 0; g < G; ++g) o[g] = issue_row<T, WIDE>(row, n0 + g * KC + q * E, a.N);
+            for (int i = 0; i < LP; ++i) {
+                const int64_t m = m0 + i * (64 / VP) + lane / VP;
+                o[i] = issue_row<T, WIDE>(other + (whole.value || m < end ? m : end - 1) * a.ldo, n0 + lane % VP * E,
+                                          a.N);
+            }
         }
-        if constexpr (whole.value) load(m + 64);
+        if constexpr (whole.value) load(m0 + 64);
+        wave_fence();
+#pragma unroll
+        for (int c = 0; c < KCH; ++c) xf[c] = mine[r * PK + c * 4 + q];
+        wave_fence();
+        if constexpr (EPI != 0) {
+#pragma unroll
+            for (int i = 0; i < LP; ++i) {
+                u32x4 v = o[i];
+                if (n0 + VP * E > a.N) v = finish_row<T, WIDE>(v, n0 + lane % VP * E, a.N);
+                mine[(i * (64 / VP) + lane / VP) * PO + lane % VP] = v;
+            }
+            wave_fence();
+        }
         // The weights stay in LDS: hoisted out of the loop they would take
         // every register (128 at 4 chunks x 8 tiles).
-        int mine = lane;
-        asm volatile("" : "+v"(mine));
+        int at_w = lane;
+        asm volatile("" : "+v"(at_w));
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             if (sizeof(T) == 4 && n0 + g * KC >= a.N) break;
             f32x4 acc[TG];
 #pragma unroll
-            for (int t = 0; t < TG; ++t) acc[t] = bias_lds[g * 4 * TG + (mine >> 4) * TG + t];
+            for (int t = 0; t < TG; ++t) acc[t] = bias_lds[g * 4 * TG + (at_w >> 4) * TG + t];
 #pragma unroll
             for (int c = 0; c < KCH; ++c)
 #pragma unroll
                 for (int t = 0; t < TG; ++t)
-                    acc[t] = multiply_chunk<T>(w_lds[(c * NT + g * TG + t) * 64 + mine], xf[c], acc[t], a.K - c * KC);
+                    acc[t] = multiply_chunk<T>(w_lds[(c * NT + g * TG + t) * 64 + at_w], xf[c], acc[t], a.K - c * KC);
             settle(acc);
-            const int at = n0 + g * KC;
             float z[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) z[i] = acc[i / 4][i & 3];
+            u32x4& slot = mine[r * PO + g * 4 + q];
             u32x4 raw = {0u, 0u, 0u, 0u};
-            if constexpr (EPI != 0) raw = finish_chunk<T, WIDE>(o[g], at, at + q * E, a.N);
+            if constexpr (EPI != 0) raw = slot;
             raw = linear_end<T, EPI, E>(a, z, raw);
-            if (staged) out_lds[wave][r * PO + g * 4 + q] = raw;
-            else if (whole.value || m < end) store_chunk(y + m * a.N, at, at + q * E, a.N, raw);
+            const int64_t m = m0 + r;
+            if (staged) slot = raw;
+            else if (whole.value || m < end) store_chunk(y + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
         }
-        if (!staged) return;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const int vec = lane % VP, at = n0 + vec * E;
-#pragma unroll
-        for (int i = 0; i < 16 * VP / 64; ++i) {
-            const int row = i * (64 / VP) + lane / VP;
-            const u32x4 raw = out_lds[wave][row * PO + vec];
-            const int64_t to = m - r + row;
-            if (whole.value && n0 + 16 * NT <= a.N) store16(y + to * a.N + at, raw);
-            else if (to < end) store_row(y + to * a.N, at, a.N, raw);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        if (staged) store_strip<T, VP, PO>(mine, y, m0, end, n0, a.N, lane, whole);
+        else wave_fence();
     };
-    int64_t m = first + wave * 16 + r;
-    load(m);
-    for (; m - r + 16 <= end; m += 64) strip(m, Flag<true>{});
-    if (m - r < end) strip(m, Flag<false>{});
+    for (; m0 + 16 <= end; m0 += 64) strip(m0, Flag<true>{});
+    if (m0 < end) strip(m0, Flag<false>{});
 }
 
 // Longer contracted dimensions, where the products count more than the bytes:
@@ -208,7 +246,10 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     constexpr int WL = (CH * NT + 3) / 4;  // fragment vectors of W a thread brings in
     constexpr int TG = KC / 16;
     constexpr int G = NT / TG;
-    __shared__ u32x4 w_lds[2][CH * NT * 64];
+    constexpr int VP = 16 * NT / E, PO = VP + 1;  // an output row's vectors, and its pitch in LDS
+    constexpr int STEP = CH * NT * 64;            // fragment vectors of a step's weights
+    constexpr int OUT = 4 * 16 * PO;
+    __shared__ u32x4 lds[2 * STEP > OUT ? 2 * STEP : OUT];  // the weights' two buffers, then the outputs
     __shared__ float bias_lds[16 * NT];
 
     int64_t row_block;
@@ -254,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
             if (CH * NT % 4 != 0 && slot >= CH * NT * 64) break;
             const int c = slot / (NT * 64), t = (slot / 64) % NT, l = slot & 63;
             const u32x4 v = finish_chunk<T, WIDE>(wr[i], k0 + c * KC, k0 + c * KC + (l >> 4) * E, a.K);
-            w_lds[buffer][slot] = n0 + tile_column<T>(t, l & 15) < a.N ? v : u32x4{0u, 0u, 0u, 0u};
+            lds[buffer * STEP + slot] = n0 + tile_column<T>(t, l & 15) < a.N ? v : u32x4{0u, 0u, 0u, 0u};
         }
     };
 
@@ -280,7 +321,7 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const u32x4 wf = w_lds[buffer][(c * NT + t) * 64 + lane];
+                const u32x4 wf = lds[buffer * STEP + (c * NT + t) * 64 + lane];
 #pragma unroll
                 for (int s = 0; s < RS; ++s) acc[s][t] = multiply<T>(wf, xc[s][c], acc[s][t]);
             }
@@ -292,14 +333,17 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     for (int s = 0; s < RS; ++s) settle(acc[s]);
     T* y = static_cast<T*>(a.y);
     const T* other = static_cast<const T*>(a.other);
+    const bool staged = a.N % E == 0;
+    u32x4* strip = lds + wave * 16 * PO;
+    __syncthreads();  // the weights' last readers are done
 #pragma unroll
     for (int s = 0; s < RS; ++s) {
         const int64_t m = first + wave * (16 * RS) + 16 * s + r;
-        if (m >= a.rows) continue;
+        const int64_t at_row = m < a.rows ? m : a.rows - 1;
         u32x4 o[G];
         if constexpr (EPI != 0) {
 #pragma unroll
-            for (int g = 0; g < G; ++g) o[g] = issue_row<T, WIDE>(other + m * a.ldo, n0 + g * KC + q * E, a.N);
+            for (int g = 0; g < G; ++g) o[g] = issue_row<T, WIDE>(other + at_row * a.ldo, n0 + g * KC + q * E, a.N);
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -309,7 +353,178 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
             for (int i = 0; i < E; ++i) z[i] = acc[s][g * TG + i / 4][i & 3] + bias_lds[at + i];
             u32x4 raw = {0u, 0u, 0u, 0u};
             if constexpr (EPI != 0) raw = finish_chunk<T, WIDE>(o[g], n0 + g * KC, n0 + at, a.N);
-            store_chunk(y + m * a.N, n0 + g * KC, n0 + at, a.N, linear_end<T, EPI, E>(a, z, raw));
+            raw = linear_end<T, EPI, E>(a, z, raw);
+            if (staged) strip[r * PO + g * 4 + q] = raw;
+            else if (m < a.rows) store_chunk(y + m * a.N, n0 + g * KC, n0 + at, a.N, raw);
+        }
+        if (staged) {
+            if (m - r + 16 <= a.rows) store_strip<T, VP, PO>(strip, y, m - r, a.rows, n0, a.N, lane, Flag<true>{});
+            else store_strip<T, VP, PO>(strip, y, m - r, a.rows, n0, a.N, lane, Flag<false>{});
+        }
+    }
+}
+
+// The weights as the tile kernel takes them: fragments of W (or of W^T), 64
+// columns (4 tiles) after 64, within them chunk by chunk, zero past N and K, so
+// that a wavefront reads a fragment as 1 KB in a row.
+template <class T, bool TRANSPOSED>
+__global__ __launch_bounds__(256) void pack_weights_kernel(const T* __restrict__ w, int N, int K, int chunks,
+                                                           u32x4* __restrict__ out) {
+    constexpr int E = VEC<T>;
+    const int slot = blockIdx.x * 256 + threadIdx.x;
+    const int l = slot & 63, t = (slot >> 6) & 3, rest = slot >> 8;
+    const int c = rest % chunks, n = rest / chunks * 64 + tile_column<T>(t, l & 15);
+    const int k = c * CHUNK<T> + (l >> 4) * E;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (n < N) {
+        if constexpr (!TRANSPOSED) {
+            v = load_row(w + (int64_t)n * K, k, K);
+        } else {
+            float f[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] = k + i < K ? to_f32(w[(int64_t)(k + i) * N + n]) : 0.0f;
+            v = pack<T>(f);
+        }
+    }
+    out[slot] = v;
+}
+template <class T>
+static int64_t packed_vectors(int N, int K) {
+    return (int64_t)((N + 63) / 64) * ((K + CHUNK<T> - 1) / CHUNK<T>) * 256;
+}
+
+// Longer contracted dimensions with many rows: a block of 4 wavefronts brings
+// 64 whole rows of x into LDS and goes over all N columns: a wavefront takes 64
+// of them at a time against the 64 rows (4 x 4 tiles), its fragments of W,
+// packed, from the L2, where they stay.  After the rows have come the
+// wavefronts never wait for one another.  TILE_NOTE
+template <class T, bool Q8, int EPI, int KCH>
+__global__ __launch_bounds__(256, KCH * (int)sizeof(T) > 64 ? 1 : 2)
+void linear_tile_kernel(LinearRows a) {
+    constexpr int E = VEC<T>;
+    constexpr int KC = CHUNK<T>;
+    constexpr int TG = KC / 16;
+    constexpr int NT = 4, G = NT / TG;
+    constexpr int PAD = sizeof(T) == 4 ? 1 : 2;
+    constexpr int VK = KCH * 4, PK = VK + PAD;
+    constexpr int VP = 16 * NT / E, PO = VP + PAD;
+    constexpr int LP = 16 * VP / 64;
+    constexpr int LK = 64 * VK / 256;    // vectors of x a thread brings in
+    constexpr int LB = LK < 8 ? LK : 8;  // of which this many at a time
+    __shared__ u32x4 x_lds[64 * PK];
+    __shared__ u32x4 strip_lds[4][16 * PO];
+
+    const int64_t first = (int64_t)blockIdx.x * 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const int r = lane & 15, q = lane >> 4;
+    const u32x4* w = static_cast<const u32x4*>(a.w);
+    const T* bias = static_cast<const T*>(a.bias);
+    const T* other = static_cast<const T*>(a.other);
+    T* y = static_cast<T*>(a.y);
+    u32x4* mine = strip_lds[wave];
+
+#pragma unroll
+    for (int b = 0; b < LK; b += LB) {
+        RowRaw<T, Q8, true> xr[LB];
+#pragma unroll
+        for (int i = 0; i < LB; ++i) {
+            const int u = (b + i) * 256 + tid;
+            const int64_t m = first + u / VK < a.rows ? first + u / VK : a.rows - 1;
+            xr[i].issue(a.x, m, u % VK * E);
+        }
+#pragma unroll
+        for (int i = 0; i < LB; ++i) {
+            const int u = (b + i) * 256 + tid;
+            x_lds[u / VK * PK + u % VK] = xr[i].finish_in(a.x, VK * E <= a.K, u % VK * E);
+        }
+    }
+    __syncthreads();
+
+    const bool staged = a.N % E == 0;
+    const int chunks = (a.K + KC - 1) / KC;
+    for (int n0 = wave * 64; n0 < a.N; n0 += 256) {
+        f32x4 acc[4][NT];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[s][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        // Two chunks of W are on their way while one is multiplied.
+        const u32x4* from = w + (int64_t)(n0 / 64) * chunks * 256 + lane;
+        u32x4 next[2][NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            next[0][t] = from[t * 64];
+            next[1][t] = from[(chunks > 1 ? 256 : 0) + t * 64];
+        }
+        auto step = [&](int c, u32x4 (&wf)[NT]) {
+            u32x4 cur[NT], xf[4];
+            const int ahead = c + 2 < chunks ? c + 2 : chunks - 1;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                cur[t] = wf[t];
+                wf[t] = from[ahead * 256 + t * 64];
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) xf[s] = x_lds[(16 * s + r) * PK + c * 4 + q];
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[s][t] = multiply<T>(cur[t], xf[s], acc[s][t]);
+        };
+        for (int c = 0; c < chunks; c += 2) {
+            step(c, next[0]);
+            if (c + 1 < chunks) step(c + 1, next[1]);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) settle(acc[s]);
+        float add[G][E];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            if (bias) {
+                unpack<T>(load_row(bias, n0 + g * KC + q * E, a.N), add[g]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) add[g][i] = 0.0f;
+            }
+        }
+        auto finish = [&](int s, auto whole) {
+            const int64_t m0 = first + 16 * s, m = m0 + r;
+            if constexpr (EPI != 0) {
+                u32x4 o[LP];
+#pragma unroll
+                for (int i = 0; i < LP; ++i) {
+                    const int64_t at = m0 + i * (64 / VP) + lane / VP;
+                    o[i] = issue_row<T, true>(other + (whole.value || at < a.rows ? at : a.rows - 1) * a.ldo,
+                                              n0 + lane % VP * E, a.N);
+                }
+#pragma unroll
+                for (int i = 0; i < LP; ++i) {
+                    u32x4 v = o[i];
+                    if (n0 + VP * E > a.N) v = finish_row<T, true>(v, n0 + lane % VP * E, a.N);
+                    mine[(i * (64 / VP) + lane / VP) * PO + lane % VP] = v;
+                }
+                wave_fence();
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float z[E];
+#pragma unroll
+                for (int i = 0; i < E; ++i) z[i] = acc[s][g * TG + i / 4][i & 3] + add[g][i];
+                u32x4& slot = mine[r * PO + g * 4 + q];
+                u32x4 raw = {0u, 0u, 0u, 0u};
+                if constexpr (EPI != 0) raw = slot;
+                raw = linear_end<T, EPI, E>(a, z, raw);
+                if (staged) slot = raw;
+                else if (whole.value || m < a.rows)
+                    store_chunk(y + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
+            }
+            if (staged) store_strip<T, VP, PO>(mine, y, m0, a.rows, n0, a.N, lane, whole);
+            else wave_fence();
+        };
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (first + 16 * s + 16 <= a.rows) finish(s, Flag<true>{});
+            else if (first + 16 * s < a.rows) finish(s, Flag<false>{});
         }
     }
 }
@@ -528,16 +743,45 @@ static void launch_stream(const LinearRows& a, hipStream_t stream) {
     else if (a.N <= 64) launch_stream_as<T, Q8, EPI, KCH, 4, true>(a, stream);
     else launch_stream_as<T, Q8, EPI, KCH, 8, true>(a, stream);
 }
-template <class T, bool Q8, int EPI>
-static void launch_long(const LinearRows& a, hipStream_t stream) {
-    if (a.N < VEC<T>) launch_long_as<T, Q8, EPI, 1, 2, false>(a, stream);
-    else if (few_rows(a)) launch_long_as<T, Q8, EPI, 1, 2, true>(a, stream);
-    else if (a.N <= 32) launch_long_as<T, Q8, EPI, 4, 2, true>(a, stream);
-    else if (a.N <= 64) launch_long_as<T, Q8, EPI, 4, 4, true>(a, stream);
-    else launch_long_as<T, Q8, EPI, 4, 8, true>(a, stream);
+// Products that the tile kernel takes: more than 4 chunks of K, as many as a
+// block's rows find room for, and enough rows to fill the blocks.
+template <class T>
+static bool tiled(int64_t rows, int K, int N) {
+    return K > 4 * CHUNK<T> && K <= 512 && rows > 1024 && N >= VEC<T>;
+}
+template <class T, bool Q8, int EPI, int KCH>
+static void launch_tile(const LinearRows& a, hipStream_t stream) {
+    hipLaunchKernelGGL((linear_tile_kernel<T, Q8, EPI, KCH>), dim3((unsigned)((a.rows + 63) / 64)), dim3(256), 0,
+                       stream, a);
 }
 template <class T, bool Q8, int EPI>
-static void launch_rows(const LinearRows& a, hipStream_t stream) {
+static void launch_long(const LinearRows& a, hipStream_t stream) {
+    if (a.N < VEC<T>) return launch_long_as<T, Q8, EPI, 1, 2, false>(a, stream);
+    if (few_rows(a)) return launch_long_as<T, Q8, EPI, 1, 2, true>(a, stream);
+    if (a.N <= 64) launch_long_as<T, Q8, EPI, 4, 4, true>(a, stream);
+    else launch_long_as<T, Q8, EPI, 2, 8, true>(a, stream);
+}
+// `packed`: room for the packed weights where the tile kernel takes the
+// product; TRANSPOSED: a.w is K x N.
+template <class T, bool Q8, int EPI, bool TRANSPOSED>
+static void launch_rows(LinearRows a, void* packed, hipStream_t stream) {
+    if (tiled<T>(a.rows, a.K, a.N)) {
+        const int64_t vectors = packed_vectors<T>(a.N, a.K);
+        hipLaunchKernelGGL((pack_weights_kernel<T, TRANSPOSED>), dim3((unsigned)(vectors / 256)), dim3(256), 0, stream,
+                           static_cast<const T*>(a.w), a.N, a.K, (a.K + CHUNK<T> - 1) / CHUNK<T>,
+                           static_cast<u32x4*>(packed));
+        a.w = packed;
+        const int chunks = (a.K + CHUNK<T> - 1) / CHUNK<T>;
+        if (chunks <= 8) return launch_tile<T, Q8, EPI, 8>(a, stream);
+        if (chunks <= 16) return launch_tile<T, Q8, EPI, 16>(a, stream);
+        if constexpr (sizeof(T) == 4) return launch_tile<T, Q8, EPI, 32>(a, stream);
+    }
+    if constexpr (TRANSPOSED) {
+        T* wt = static_cast<T*>(packed);
+        hipLaunchKernelGGL(transpose_kernel<T>, dim3((a.N + 31) / 32, (a.K + 31) / 32), dim3(256), 0, stream,
+                           static_cast<const T*>(a.w), a.K, a.N, wt);
+        a.w = wt;
+    }
     switch (chunks_of<T>(a.K)) {
         case 1: return launch_stream<T, Q8, EPI, 1>(a, stream);
         case 2: return launch_stream<T, Q8, EPI, 2>(a, stream);
@@ -604,18 +848,26 @@ static BwdScratch bwd_scratch(int64_t rows, int K, int N) {
     s.part = 0;
     s.dz = aligned((size_t)p.splits * ((size_t)N * K + N) * 4);
     s.wt = s.dz + (p.fused ? 0 : aligned((size_t)rows * N * sizeof(T)));
-    s.total = s.wt + (p.fused ? 0 : aligned((size_t)N * K * sizeof(T)));
+    // W^T as it is, or packed; W packed in its place before.
+    const size_t packed = (size_t)(packed_vectors<T>(N, K) > packed_vectors<T>(K, N) ? packed_vectors<T>(N, K)
+                                                                                       : packed_vectors<T>(K, N)) * 16;
+    s.total = s.wt + (p.fused ? 0 : aligned(packed));
     return s;
 }
 
 template <class T>
-static int linear_fwd(const gs3d_linear_args& g, hipStream_t stream) {
+static size_t fwd_bytes(int64_t rows, int K, int N) {
+    return tiled<T>(rows, K, N) ? (size_t)packed_vectors<T>(N, K) * 16 : 0;
+}
+
+template <class T>
+static int linear_fwd(const gs3d_linear_args& g, void* scratch, hipStream_t stream) {
     LinearRows a{};
     a.x = Rows{g.x, g.x_stride, {}, g.inner};
     a.w = g.weight, a.bias = g.bias, a.other = g.residual, a.ldo = g.residual_stride, a.y = g.y;
     a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
-    if (g.residual) launch_rows<T, false, 2>(a, stream);
-    else launch_rows<T, false, 0>(a, stream);
+    if (g.residual) launch_rows<T, false, 2, false>(a, scratch, stream);
+    else launch_rows<T, false, 0, false>(a, scratch, stream);
     return launch_status("gs3d_linear_fwd");
 }
 
@@ -645,18 +897,15 @@ static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t 
             a.x = x, a.w = g.weight, a.bias = g.bias, a.other = g.upstream, a.ldo = g.upstream_stride;
             a.y = scratch + at.dz;
             a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
-            launch_rows<T, Q8, 1>(a, stream);
+            launch_rows<T, Q8, 1, false>(a, scratch + at.wt, stream);
             dz = scratch + at.dz;
             ldz = g.outer;
         }
         if (g.grad_x && g.rows > 0) {
-            T* wt = reinterpret_cast<T*>(scratch + at.wt);
-            hipLaunchKernelGGL(transpose_kernel<T>, dim3((g.inner + 31) / 32, (g.outer + 31) / 32), dim3(256), 0,
-                               stream, static_cast<const T*>(g.weight), g.outer, g.inner, wt);
             LinearRows a{};
-            a.x = Rows{dz, ldz, {}, g.outer}, a.w = wt, a.y = g.grad_x;
+            a.x = Rows{dz, ldz, {}, g.outer}, a.w = g.weight, a.y = g.grad_x;
             a.rows = g.rows, a.K = g.outer, a.N = g.inner, a.act = GS3D_ACT_NONE;
-            launch_rows<T, false, 0>(a, stream);
+            launch_rows<T, false, 0, true>(a, scratch + at.wt, stream);
         }
         if (params) {
             LinearGradW a{x, dz, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, part, g.inner};

@@ -31,7 +31,9 @@ class _Linear(torch.autograd.Function):
             residual, a.residual_stride = rows_of(residual)
             a.residual = native.ptr(residual)
         if a.rows:
-            launch("gs3d_linear_fwd", ctypes.byref(a), x.device)
+            nbytes = native.query("gs3d_linear_fwd_scratch_bytes", a.rows, inner, outer, a.dtype)
+            work = scratch(nbytes, x.device) if nbytes else None
+            launch("gs3d_linear_fwd", ctypes.byref(a), x.device, native.ptr(work), nbytes)
         if grad_enabled and any(ctx.needs_input_grad[:3]):
             # The input is needed for the weight's gradient and for the slope
             # of an activation; without either it is not kept.

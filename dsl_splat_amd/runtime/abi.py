@@ -397,7 +397,8 @@ FUNCTIONS = {
     "gs3d_render_fwd_stats": (ctypes.c_int, [ctypes.POINTER(RenderArgs), ctypes.POINTER(RenderStatsArgs), _P]),
     "gs3d_render_bwd": (ctypes.c_int, [ctypes.POINTER(RenderBwdArgs), _P]),
     "gs3d_render_bwd_lists": (ctypes.c_int, [ctypes.POINTER(RenderBwdArgs), _I64, _P]),
-    "gs3d_linear_fwd": (ctypes.c_int, [ctypes.POINTER(LinearArgs), _P]),
+    "gs3d_linear_fwd_scratch_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
+    "gs3d_linear_fwd": (ctypes.c_int, [ctypes.POINTER(LinearArgs), _P, _SZ, _P]),
     "gs3d_linear_bwd_scratch_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
     "gs3d_linear_bwd": (ctypes.c_int, [ctypes.POINTER(LinearBwdArgs), _P, _SZ, _P]),
     "gs3d_group_norm_scratch_bytes": (_SZ, [_I32, _I64, _I32, _I32, _I32]),

@@ -559,7 +559,9 @@ enum { GS3D_ACT_NONE = 0, GS3D_ACT_RELU = 1, GS3D_ACT_SILU = 2, GS3D_ACT_GELU = 
 #define GS3D_MAX_IMAGES 65535
 
 /* y = act(x W^T + bias) + residual: x (rows, inner), W (outer, inner), y
- * (rows, outer).  bias and residual may be NULL. */
+ * (rows, outer).  bias and residual may be NULL.  Scratch:
+ * gs3d_linear_fwd_scratch_bytes (16-byte aligned; 0 for most sizes, then
+ * scratch may be NULL). */
 typedef struct gs3d_linear_args {
     int64_t rows;
     int32_t inner, outer;
@@ -573,14 +575,15 @@ typedef struct gs3d_linear_args {
     void* y;
 } gs3d_linear_args;
 
-int gs3d_linear_fwd(const gs3d_linear_args* args, void* stream);
+size_t gs3d_linear_fwd_scratch_bytes(int64_t rows, int32_t inner, int32_t outer, int32_t dtype);
+int gs3d_linear_fwd(const gs3d_linear_args* args, void* scratch, size_t scratch_bytes, void* stream);
 
 /* Gradients of gs3d_linear_fwd from upstream = dL/dy (the residual's gradient
  * is upstream itself): with z = x W^T + bias and dz = upstream act'(z), z
  * computed again, grad_x = dz W, grad_weight = dz^T x, grad_bias = sum dz;
  * each may be NULL.  The input is either x or, in 8 bits, codes and scales
  * (gs3d_quantize_activations; x NULL then), which stand for x everywhere.
- * Scratch: gs3d_linear_bwd_scratch_bytes. */
+ * Scratch: gs3d_linear_bwd_scratch_bytes, 16-byte aligned. */
 typedef struct gs3d_linear_bwd_args {
     int64_t rows;
     int32_t inner, outer;
@@ -605,7 +608,8 @@ int gs3d_linear_bwd(const gs3d_linear_bwd_args* args, void* scratch, size_t scra
  * mean and variance per image and group of channels / groups neighbouring
  * channels, rstd = 1 / sqrt(variance + eps).  weight and bias may be NULL.
  * statistics (images, groups, 2) receives mean and rstd for the backward
- * pass.  Scratch: gs3d_group_norm_scratch_bytes, in both directions. */
+ * pass.  Scratch: gs3d_group_norm_scratch_bytes, 16-byte aligned, in both
+ * directions. */
 typedef struct gs3d_group_norm_args {
     int32_t images;
     int64_t pixels;

@@ -40,7 +40,7 @@ def _norm_bwd():
 
 
 @pytest.mark.parametrize("make,name,scratch,changes", [
-    (_linear, "gs3d_linear_fwd", False, [
+    (_linear, "gs3d_linear_fwd", True, [
         ("rows", -1), ("rows", abi.MAX_ROWS + 1), ("inner", 0), ("outer", 0), ("inner", abi.MAX_CHANNELS + 1),
         ("dtype", 3), ("dtype", -1), ("activation", 4), ("activation", -1), ("x_stride", 7), ("x", None),
         ("weight", None), ("y", None)]),
@@ -58,7 +58,7 @@ def _norm_bwd():
 ])
 def test_entry_points_check_their_arguments(make, name, scratch, changes):
     call = getattr(native.load(), name)
-    more = (P, 1 << 40) if scratch else ()
+    more = (P, 1 << 40)
     for field, value in changes:
         a = make()
         setattr(a, field, value)
@@ -66,6 +66,8 @@ def test_entry_points_check_their_arguments(make, name, scratch, changes):
     assert call(None, *more, None) == abi.GS3D_ERR_ARGUMENT
     if scratch:
         a = make()
+        if name == "gs3d_linear_fwd":
+            a.rows, a.inner, a.x_stride = 100_000, 300, 300  # packed weights
         assert call(ctypes.byref(a), P, 1, None) == abi.GS3D_ERR_SCRATCH
         assert call(ctypes.byref(a), None, 1 << 40, None) == abi.GS3D_ERR_SCRATCH
 
@@ -91,7 +93,7 @@ def test_scratch_queries():
     # Empty work is a no-op.
     a = _linear()
     a.rows, a.x, a.weight, a.y = 0, None, None, None
-    assert native.load().gs3d_linear_fwd(ctypes.byref(a), None) == abi.GS3D_OK
+    assert native.load().gs3d_linear_fwd(ctypes.byref(a), None, 0, None) == abi.GS3D_OK
     n = _norm()
     n.pixels, n.x, n.y, n.statistics = 0, None, None, None
     assert native.load().gs3d_group_norm_fwd(ctypes.byref(n), None, 0, None) == abi.GS3D_OK
