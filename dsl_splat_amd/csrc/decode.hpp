@@ -286,6 +286,71 @@ GS3D_DEV int q8_code(float v, float inverse) {
 // so reaches the scale byte (the hardware's float maximum drops it).
 GS3D_DEV uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
+// Largest of the magnitudes in the lanes that share a block: a quad, or with
+// LANES = 8 two quads.  They all must be active.
+template <int LANES>
+GS3D_DEV uint32_t q8_block_max(uint32_t v) {
+    uint32_t o = dpp_u<0xB1>(v);  // quad_perm [1,0,3,2]
+    v = v > o ? v : o;
+    o = dpp_u<0x4E>(v);  // quad_perm [2,3,0,1]
+    v = v > o ? v : o;
+    if constexpr (LANES == 8) {
+        o = dpp_u<0x141>(v);  // row_half_mirror: the other quad of the eight
+        v = v > o ? v : o;
+    }
+    return v;
+}
+
+// Four codes as a word.
+GS3D_DEV uint32_t q8_word(const float* v, uint32_t byte) {
+    uint32_t word = 0u;
+    if (byte != 255u) {
+        const float inverse = q8_inverse_scale(byte);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) word |= ((uint32_t)q8_code(v[i], inverse) & 0xFFu) << (8 * i);
+    }
+    return word;
+}
+
+// Codes from `at` on of a row of `count`: N words of four.
+template <int N>
+GS3D_DEV void q8_store(int8_t* row, int at, int count, const uint32_t (&words)[N]) {
+    if (at + 4 * N <= count) {
+        if constexpr (N == 2) *reinterpret_cast<u32x2_at1*>(row + at) = u32x2{words[0], words[1]};
+        else *reinterpret_cast<u32_at1*>(row + at) = words[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i)
+            if (at + i < count) row[at + i] = (int8_t)(words[i / 4] >> (8 * (i & 3)));
+    }
+}
+
+// One lane's vector of a row written in 8 bits, from channel `at` on; 32 /
+// VEC<T> neighbouring lanes, all active, hold a block (zeros past the row's
+// end).  `live`: the row is there.
+template <class T>
+GS3D_DEV void q8_keep(const float (&v)[VEC<T>], int8_t* codes, uint8_t* scales, int64_t row, int at, int channels,
+                      bool live) {
+    constexpr int E = VEC<T>;
+    uint32_t largest = 0u;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const uint32_t m = magnitude_bits(v[i]);
+        largest = m > largest ? m : largest;
+    }
+    const uint32_t byte = q8_scale_byte<T>(q8_block_max<32 / E>(largest));
+    uint32_t words[E / 4];
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) words[i] = q8_word(v + 4 * i, byte);
+    if (!live || at >= channels) return;
+    q8_store(codes + row * channels, at, channels, words);
+    if ((at & 31) == 0) scales[row * ((channels + 31) >> 5) + (at >> 5)] = (uint8_t)byte;
+}
+
+// Rows of a strided tensor in 8 bits, a launch of its own (quantize.hip).
+void quantize_rows(const void* x, int64_t ldx, int64_t rows, int channels, int dtype, int8_t* codes, uint8_t* scales,
+                   hipStream_t stream);
+
 struct Q8Rows {
     const int8_t* codes;    // rows x channels
     const uint8_t* scales;  // rows x blocks of 32 channels

@@ -180,8 +180,11 @@ __global__ __launch_bounds__(1024) void norm_merge_kernel(NormShape s, const flo
     }
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, Rows a, NormParams p, T* __restrict__ y) {
+// KEEP: x is also written in 8 bits as it is read; whole blocks of 32 channels
+// then, so that a block lies in neighbouring lanes.
+template <class T, bool KEEP>
+__global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, Rows a, NormParams p, T* __restrict__ y,
+                                                         int8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     constexpr int E = VEC<T>;
     constexpr int U = 4;
     const NormThread t = norm_thread<E>(s.channels);
@@ -203,6 +206,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, Rows a, No
             if (at >= end) break;
             float v[E];
             unpack<T>(raw[k].finish(a, t.at), v);
+            if constexpr (KEEP) q8_keep<T>(v, codes, scales, base + at, t.at, s.channels, true);
 #pragma unroll
             for (int i = 0; i < E; ++i) v[i] = __builtin_fmaf(v[i] - mean[i], scale[i], beta[i]);
             activate(v, s.act);
@@ -438,8 +442,15 @@ static int norm_fwd(const gs3d_group_norm_args& g, void* scratch, hipStream_t st
     const dim3 grid = norm_grid(s, g.dtype);
     hipLaunchKernelGGL(norm_statistics_kernel<T>, grid, dim3(256), 0, stream, s, a, part);
     hipLaunchKernelGGL(norm_merge_kernel, dim3(s.groups, s.images), dim3(1024), 0, stream, s, part, stats);
-    hipLaunchKernelGGL(norm_apply_kernel<T>, grid, dim3(256), 0, stream, s, a, NormParams{g.weight, g.bias, stats},
-                       static_cast<T*>(g.y));
+    const NormParams p{g.weight, g.bias, stats};
+    T* y = static_cast<T*>(g.y);
+    if (g.codes && g.channels % Q8_BLOCK == 0) {
+        hipLaunchKernelGGL((norm_apply_kernel<T, true>), grid, dim3(256), 0, stream, s, a, p, y, g.codes, g.scales);
+    } else {
+        if (g.codes)
+            quantize_rows(g.x, g.x_stride, g.images * g.pixels, g.channels, g.dtype, g.codes, g.scales, stream);
+        hipLaunchKernelGGL((norm_apply_kernel<T, false>), grid, dim3(256), 0, stream, s, a, p, y, nullptr, nullptr);
+    }
     return launch_status("gs3d_group_norm_fwd");
 }
 
@@ -488,7 +499,7 @@ extern "C" int gs3d_group_norm_fwd(const gs3d_group_norm_args* g, void* scratch,
         !(g->eps > 0.0f) || g->x_stride < g->channels)
         return GS3D_ERR_ARGUMENT;
     if (g->images == 0 || g->pixels == 0) return GS3D_OK;
-    if (!g->x || !g->y || !g->statistics) return GS3D_ERR_ARGUMENT;
+    if (!g->x || !g->y || !g->statistics || !g->codes != !g->scales) return GS3D_ERR_ARGUMENT;
     if (!scratch ||
         scratch_bytes < gs3d_group_norm_scratch_bytes(g->images, g->pixels, g->channels, g->groups, g->dtype))
         return GS3D_ERR_SCRATCH;

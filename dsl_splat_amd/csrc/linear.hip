@@ -35,7 +35,7 @@ extern "C" int gs3d_linear_fwd(const gs3d_linear_args* g, void* scratch, size_t 
     if (!g || !gs3d::linear_sizes_ok(g->rows, g->inner, g->outer, g->dtype, g->activation)) return GS3D_ERR_ARGUMENT;
     if (g->x_stride < g->inner || (g->residual && g->residual_stride < g->outer)) return GS3D_ERR_ARGUMENT;
     if (g->rows == 0) return GS3D_OK;
-    if (!g->x || !g->weight || !g->y) return GS3D_ERR_ARGUMENT;
+    if (!g->x || !g->weight || !g->y || !g->codes != !g->scales) return GS3D_ERR_ARGUMENT;
     const size_t needed = gs3d_linear_fwd_scratch_bytes(g->rows, g->inner, g->outer, g->dtype);
     if (needed > 0 && (!scratch || scratch_bytes < needed)) return GS3D_ERR_SCRATCH;
     const hipStream_t s = gs3d::as_stream(stream);

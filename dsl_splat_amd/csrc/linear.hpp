@@ -33,6 +33,8 @@ struct LinearRows {
     void* y;             // rows x N
     int64_t rows;
     int K, N, act, n_tiles, strips;
+    int8_t* keep_codes;  // where the rows of x are kept in 8 bits, or NULL
+    uint8_t* keep_scales;
 };
 
 // Blocks b, b + 8, b + 16, ... run on one XCD: the column tiles of a range of
@@ -169,11 +171,22 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
     __syncthreads();
 
     const bool staged = a.N % E == 0;  // else segments start anywhere, and vectors leave as they come
+    const bool keep = a.keep_codes && n_tile == 0;
     auto strip = [&](int64_t m0, auto whole) {
         u32x4 xf[KCH];
 #pragma unroll
-        for (int i = 0; i < LK; ++i)
-            mine[(i * (64 / VK) + lane / VK) * PK + lane % VK] = xr[i].finish_in(a.x, VK * E <= a.K, lane % VK * E);
+        for (int i = 0; i < LK; ++i) {
+            const u32x4 v = xr[i].finish_in(a.x, VK * E <= a.K, lane % VK * E);
+            mine[(i * (64 / VK) + lane / VK) * PK + lane % VK] = v;
+            if constexpr (EPI != 1 && !Q8) {
+                if (keep) {
+                    const int64_t m = m0 + i * (64 / VK) + lane / VK;
+                    float f[E];
+                    unpack<T>(v, f);
+                    q8_keep<T>(f, a.keep_codes, a.keep_scales, m, lane % VK * E, a.K, whole.value || m < end);
+                }
+            }
+        }
         u32x4 o[LP];
         if constexpr (EPI != 0) {
 #pragma unroll
@@ -399,7 +412,7 @@ static int64_t packed_vectors(int N, int K) {
 // packed, from the L2, where they stay.  After the rows have come the
 // wavefronts never wait for one another.  TILE_NOTE
 template <class T, bool Q8, int EPI, int KCH>
-__global__ __launch_bounds__(256, KCH * (int)sizeof(T) > 64 ? 1 : 2)
+__global__ __launch_bounds__(256, KCH * (int)sizeof(T) > 64 ? 1 : KCH * (int)sizeof(T) > 16 || EPI != 0 ? 2 : 3)
 void linear_tile_kernel(LinearRows a) {
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
@@ -448,32 +461,28 @@ void linear_tile_kernel(LinearRows a) {
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[s][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        // Two chunks of W are on their way while one is multiplied.
         const u32x4* from = w + (int64_t)(n0 / 64) * chunks * 256 + lane;
-        u32x4 next[2][NT];
+        u32x4 wa[NT], wb[NT];  // one chunk of W on its way while the other is multiplied
+        auto fetch = [&](int c, u32x4 (&wf)[NT]) {
+            const u32x4* p = from + (c < chunks ? c : chunks - 1) * 256;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            next[0][t] = from[t * 64];
-            next[1][t] = from[(chunks > 1 ? 256 : 0) + t * 64];
-        }
-        auto step = [&](int c, u32x4 (&wf)[NT]) {
-            u32x4 cur[NT], xf[4];
-            const int ahead = c + 2 < chunks ? c + 2 : chunks - 1;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                cur[t] = wf[t];
-                wf[t] = from[ahead * 256 + t * 64];
-            }
+            for (int t = 0; t < NT; ++t) wf[t] = p[t * 64];
+        };
+        auto step = [&](int c, const u32x4 (&wf)[NT]) {
+            u32x4 xf[4];
 #pragma unroll
             for (int s = 0; s < 4; ++s) xf[s] = x_lds[(16 * s + r) * PK + c * 4 + q];
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) acc[s][t] = multiply<T>(cur[t], xf[s], acc[s][t]);
+                for (int t = 0; t < NT; ++t) acc[s][t] = multiply<T>(wf[t], xf[s], acc[s][t]);
         };
+        fetch(0, wa);
         for (int c = 0; c < chunks; c += 2) {
-            step(c, next[0]);
-            if (c + 1 < chunks) step(c + 1, next[1]);
+            fetch(c + 1, wb);
+            step(c, wa);
+            fetch(c + 2, wa);
+            if (c + 1 < chunks) step(c + 1, wb);
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) settle(acc[s]);
@@ -487,16 +496,21 @@ void linear_tile_kernel(LinearRows a) {
                 for (int i = 0; i < E; ++i) add[g][i] = 0.0f;
             }
         }
+        u32x4 ahead[4][EPI != 0 ? LP : 1];  // all four strips' rows of dy or the residual at once
+        if constexpr (EPI != 0) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int i = 0; i < LP; ++i) {
+                    const int64_t at = first + 16 * s + i * (64 / VP) + lane / VP;
+                    ahead[s][i] = issue_row<T, true>(other + (at < a.rows ? at : a.rows - 1) * a.ldo,
+                                                     n0 + lane % VP * E, a.N);
+                }
+        }
         auto finish = [&](int s, auto whole) {
             const int64_t m0 = first + 16 * s, m = m0 + r;
             if constexpr (EPI != 0) {
-                u32x4 o[LP];
-#pragma unroll
-                for (int i = 0; i < LP; ++i) {
-                    const int64_t at = m0 + i * (64 / VP) + lane / VP;
-                    o[i] = issue_row<T, true>(other + (whole.value || at < a.rows ? at : a.rows - 1) * a.ldo,
-                                              n0 + lane % VP * E, a.N);
-                }
+                const u32x4 (&o)[LP] = ahead[s];
 #pragma unroll
                 for (int i = 0; i < LP; ++i) {
                     u32x4 v = o[i];
@@ -866,6 +880,9 @@ static int linear_fwd(const gs3d_linear_args& g, void* scratch, hipStream_t stre
     a.x = Rows{g.x, g.x_stride, {}, g.inner};
     a.w = g.weight, a.bias = g.bias, a.other = g.residual, a.ldo = g.residual_stride, a.y = g.y;
     a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
+    // The stream kernel keeps the rows as it reads them.
+    if (g.codes && !few_rows(a) && chunks_of<T>(a.K) <= 4) a.keep_codes = g.codes, a.keep_scales = g.scales;
+    else if (g.codes) quantize_rows(g.x, g.x_stride, g.rows, g.inner, g.dtype, g.codes, g.scales, stream);
     if (g.residual) launch_rows<T, false, 2, false>(a, scratch, stream);
     else launch_rows<T, false, 0, false>(a, scratch, stream);
     return launch_status("gs3d_linear_fwd");

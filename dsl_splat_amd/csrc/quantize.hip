@@ -22,34 +22,6 @@ GS3D_DEV void load8(const T* row, int at, int count, float (&v)[8]) {
     }
 }
 
-GS3D_DEV uint32_t quad_max(uint32_t v) {
-    uint32_t o = dpp_u<0xB1>(v);  // quad_perm [1,0,3,2]
-    v = v > o ? v : o;
-    o = dpp_u<0x4E>(v);  // quad_perm [2,3,0,1]
-    return v > o ? v : o;
-}
-
-// The eight codes of v as two words.
-GS3D_DEV u32x2 q8_codes8(const float (&v)[8], uint32_t byte) {
-    u32x2 words = {0u, 0u};
-    if (byte != 255u) {
-        const float inverse = q8_inverse_scale(byte);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) words[i / 4] |= ((uint32_t)q8_code(v[i], inverse) & 0xFFu) << (8 * (i & 3));
-    }
-    return words;
-}
-
-GS3D_DEV void store_codes8(int8_t* row, int at, int count, u32x2 words) {
-    if (at + 8 <= count) {
-        *reinterpret_cast<u32x2_at1*>(row + at) = words;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (at + i < count) row[at + i] = (int8_t)(words[i / 4] >> (8 * (i & 3)));
-    }
-}
-
 template <class T>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int channels,
                                                        int8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -71,10 +43,10 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
             const uint32_t m = magnitude_bits(v[k]);
             largest = m > largest ? m : largest;
         }
-        const uint32_t byte = q8_scale_byte<T>(quad_max(largest));
-        const u32x2 words = q8_codes8(v, byte);
+        const uint32_t byte = q8_scale_byte<T>(q8_block_max<4>(largest));
+        const uint32_t words[2] = {q8_word(v, byte), q8_word(v + 4, byte)};
         if (live) {
-            store_codes8(codes + row * channels, at, channels, words);
+            q8_store(codes + row * channels, at, channels, words);
             if ((i & 3) == 0) scales[unit] = (uint8_t)byte;
         }
     }
@@ -110,6 +82,13 @@ static void launch_dequantize(const Q8Rows& q, int64_t rows, void* out, hipStrea
                        q, rows, static_cast<T*>(out));
 }
 
+void quantize_rows(const void* x, int64_t ldx, int64_t rows, int channels, int dtype, int8_t* codes, uint8_t* scales,
+                   hipStream_t stream) {
+    if (dtype == GS3D_F32) launch_quantize<float>(x, ldx, rows, channels, codes, scales, stream);
+    if (dtype == GS3D_BF16) launch_quantize<bf16_t>(x, ldx, rows, channels, codes, scales, stream);
+    if (dtype == GS3D_F16) launch_quantize<f16_t>(x, ldx, rows, channels, codes, scales, stream);
+}
+
 }  // namespace gs3d
 
 extern "C" int gs3d_quantize_activations(const void* x, int64_t x_stride, int64_t rows, int32_t channels, int32_t dtype,
@@ -117,10 +96,7 @@ extern "C" int gs3d_quantize_activations(const void* x, int64_t x_stride, int64_
     if (rows < 0 || channels < 1 || x_stride < channels || dtype < 0 || dtype > 2) return GS3D_ERR_ARGUMENT;
     if (rows == 0) return GS3D_OK;
     if (!x || !codes || !scales) return GS3D_ERR_ARGUMENT;
-    const hipStream_t s = gs3d::as_stream(stream);
-    if (dtype == GS3D_F32) gs3d::launch_quantize<float>(x, x_stride, rows, channels, codes, scales, s);
-    if (dtype == GS3D_BF16) gs3d::launch_quantize<gs3d::bf16_t>(x, x_stride, rows, channels, codes, scales, s);
-    if (dtype == GS3D_F16) gs3d::launch_quantize<gs3d::f16_t>(x, x_stride, rows, channels, codes, scales, s);
+    gs3d::quantize_rows(x, x_stride, rows, channels, dtype, codes, scales, gs3d::as_stream(stream));
     return gs3d::launch_status("gs3d_quantize_activations");
 }
 

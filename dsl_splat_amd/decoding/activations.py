@@ -34,6 +34,13 @@ class QuantizedActivations:
         return out
 
 
+def empty_quantized(x: Tensor) -> QuantizedActivations:
+    channels = x.shape[-1]
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(x.shape[:-1] + ((channels + BLOCK - 1) // BLOCK,), dtype=torch.uint8, device=x.device)
+    return QuantizedActivations(codes, scales, x.dtype)
+
+
 @native.no_grad
 def quantize_activations(x: Tensor) -> QuantizedActivations:
     """x (..., C) in 8 bits.  Per 32 neighbouring channels the scale is the
@@ -44,10 +51,9 @@ def quantize_activations(x: Tensor) -> QuantizedActivations:
     check_input("x", x, 1)
     x = x.detach()
     channels = x.shape[-1]
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(x.shape[:-1] + ((channels + BLOCK - 1) // BLOCK,), dtype=torch.uint8, device=x.device)
+    out = empty_quantized(x)
     if x.numel():
         rows, stride = rows_of(x)
         launch("gs3d_quantize_activations", native.ptr(rows), x.device, stride, x.numel() // channels, channels,
-               DTYPES[x.dtype], native.ptr(codes), native.ptr(scales))
-    return QuantizedActivations(codes, scales, x.dtype)
+               DTYPES[x.dtype], native.ptr(out.codes), native.ptr(out.scales))
+    return out

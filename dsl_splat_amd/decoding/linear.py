@@ -10,7 +10,7 @@ from torch.autograd.function import once_differentiable
 
 from ..runtime import abi, native
 from ._common import (DTYPES, activation_code, check_checkpoint, check_input, check_like, launch, rows_of, scratch)
-from .activations import quantize_activations
+from .activations import empty_quantized
 
 
 class _Linear(torch.autograd.Function):
@@ -30,20 +30,22 @@ class _Linear(torch.autograd.Function):
         if residual is not None:
             residual, a.residual_stride = rows_of(residual)
             a.residual = native.ptr(residual)
+        # The input is needed for the weight's gradient and for the slope of an
+        # activation; without either it is not kept.
+        save = grad_enabled and any(ctx.needs_input_grad[:3])
+        kept: tuple[Tensor | None, ...] = (None, None, None)
+        if save and (activation != abi.ACT_NONE or ctx.needs_input_grad[1]):
+            if checkpoint is None:
+                kept = (rows, None, None)
+            else:
+                quantized = empty_quantized(x)
+                kept = (None, quantized.codes, quantized.scales)
+                a.codes, a.scales = native.ptr(quantized.codes), native.ptr(quantized.scales)
         if a.rows:
             nbytes = native.query("gs3d_linear_fwd_scratch_bytes", a.rows, inner, outer, a.dtype)
             work = scratch(nbytes, x.device) if nbytes else None
             launch("gs3d_linear_fwd", ctypes.byref(a), x.device, native.ptr(work), nbytes)
-        if grad_enabled and any(ctx.needs_input_grad[:3]):
-            # The input is needed for the weight's gradient and for the slope
-            # of an activation; without either it is not kept.
-            if activation == abi.ACT_NONE and not ctx.needs_input_grad[1]:
-                kept = (None, None, None)
-            elif checkpoint is not None:
-                quantized = quantize_activations(rows)
-                kept = (None, quantized.codes, quantized.scales)
-            else:
-                kept = (rows, None, None)
+        if save:
             ctx.save_for_backward(*kept, weight, bias)
             ctx.shape, ctx.x_stride, ctx.activation = x.shape, x_stride, activation
         ctx.set_materialize_grads(False)

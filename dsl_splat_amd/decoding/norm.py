@@ -12,7 +12,7 @@ from torch.autograd.function import once_differentiable
 
 from ..runtime import abi, native
 from ._common import (DTYPES, activation_code, check_checkpoint, check_input, check_like, launch, rows_of, scratch)
-from .activations import quantize_activations
+from .activations import empty_quantized
 
 
 def _scratch(shape, groups: int, dtype: int, device: torch.device) -> Tensor:
@@ -35,15 +35,16 @@ class _GroupNorm(torch.autograd.Function):
         a.dtype, a.activation, a.eps = DTYPES[x.dtype], activation, eps
         a.x, a.x_stride = native.ptr(rows), x_stride
         a.weight, a.bias, a.y, a.statistics = (native.ptr(t) for t in (weight, bias, y, statistics))
+        save = grad_enabled and any(ctx.needs_input_grad[:3])
+        kept: tuple[Tensor | None, ...] = (rows, None, None)
+        if save and checkpoint is not None:
+            quantized = empty_quantized(x)
+            kept = (None, quantized.codes, quantized.scales)
+            a.codes, a.scales = native.ptr(quantized.codes), native.ptr(quantized.scales)
         if x.numel():
             work = _scratch(x.shape, groups, a.dtype, x.device)
             launch("gs3d_group_norm_fwd", ctypes.byref(a), x.device, native.ptr(work), work.numel())
-        if grad_enabled and any(ctx.needs_input_grad[:3]):
-            if checkpoint is not None:
-                quantized = quantize_activations(rows)
-                kept = (None, quantized.codes, quantized.scales)
-            else:
-                kept = (rows, None, None)
+        if save:
             ctx.save_for_backward(*kept, weight, bias, statistics)
             ctx.shape, ctx.x_stride, ctx.groups, ctx.activation = x.shape, x_stride, groups, activation
         ctx.set_materialize_grads(False)

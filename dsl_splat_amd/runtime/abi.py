@@ -264,6 +264,8 @@ class LinearArgs(ctypes.Structure):
         ("residual", _P),
         ("residual_stride", ctypes.c_int64),
         ("y", _P),
+        ("codes", _P),
+        ("scales", _P),
     ]
 
 
@@ -303,6 +305,8 @@ class GroupNormArgs(ctypes.Structure):
         ("bias", _P),
         ("y", _P),
         ("statistics", _P),
+        ("codes", _P),
+        ("scales", _P),
     ]
 
 

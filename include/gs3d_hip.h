@@ -573,6 +573,8 @@ typedef struct gs3d_linear_args {
     const void* residual;
     int64_t residual_stride;
     void* y;
+    int8_t* codes;               /* optional: x is also written in 8 bits ... */
+    uint8_t* scales;             /* ... as gs3d_quantize_activations does */
 } gs3d_linear_args;
 
 size_t gs3d_linear_fwd_scratch_bytes(int64_t rows, int32_t inner, int32_t outer, int32_t dtype);
@@ -622,6 +624,8 @@ typedef struct gs3d_group_norm_args {
     const void* bias;
     void* y;
     float* statistics;
+    int8_t* codes;               /* optional, as in gs3d_linear_args */
+    uint8_t* scales;
 } gs3d_group_norm_args;
 
 size_t gs3d_group_norm_scratch_bytes(int32_t images, int64_t pixels, int32_t channels, int32_t groups, int32_t dtype);
