@@ -498,19 +498,26 @@ GS3D_DEV void settle(f32x4 (&v)[N]) {
 // multiply() for a chunk of which only the first `valid` elements count (the
 // rest are zero), `valid` the same in the whole wavefront.  Float skips the
 // instructions that would contract zeros only: matrix instructions bound its
-// products, and 33 channels are then 36 and not 48.
+// products, and 33 channels are then 36 and not 48.  It branches, so it
+// settles (12 cycles after 32 to 128).
 template <class T>
 GS3D_DEV f32x4 multiply_chunk(u32x4 a, u32x4 b, f32x4 c, int valid) {
     if constexpr (sizeof(T) == 4) {
-        if (valid <= 0) return c;
-        if (valid < 4) {
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[0]), __uint_as_float(b[0]), c, 0, 0, 0);
-            if (valid > 1)
-                c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[1]), __uint_as_float(b[1]), c, 0, 0, 0);
-            if (valid > 2)
-                c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[2]), __uint_as_float(b[2]), c, 0, 0, 0);
-            return c;
+        f32x4 v[1] = {c};
+        if (valid >= 4) {
+            v[0] = multiply<T>(a, b, v[0]);
+            settle(v);
+        } else if (valid > 0) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                if (i < valid) {
+                    v[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), v[0], 0,
+                                                                0, 0);
+                    settle(v);
+                }
+            }
         }
+        return v[0];
     }
     return multiply<T>(a, b, c);
 }

@@ -663,6 +663,7 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
             if (sum_bias) {
 #pragma unroll
                 for (int i = 0; i < A; ++i) acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
+                settle(acc_b);
             }
         }
     }

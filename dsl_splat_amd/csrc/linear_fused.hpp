@@ -75,10 +75,6 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
     const int tid = threadIdx.x, wave = wave_id();
     const int strip = (wave & 3) * 16, half = wave >> 2;
     const int wn = wave / WK, wk = wave % WK;
-    // dW's tiles that there are; for 16-bit types all of the block's, known at
-    // compile time unless they do not share out evenly.
-    const int tiles_n = SKIP ? (a.N + 15) / 16 : NT % WN ? NT : 1 << 30;
-    const int tiles_k = SKIP ? (a.K + 15) / 16 : KT % WK ? KT : 1 << 30;
     const int64_t begin = blockIdx.x * a.rows_per_block;
     const int64_t end = begin + a.rows_per_block < a.rows ? begin + a.rows_per_block : a.rows;
     const T* w = static_cast<const T*>(a.w);
@@ -214,22 +210,24 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
         if (a.part) {
 #pragma unroll
             for (int c = 0; c < 64 / KC; ++c) {
+                // Where the tiles do not share out evenly the last one is taken
+                // again, and not stored.
                 u32x4 fz[TN], fx[TK];
 #pragma unroll
-                for (int i = 0; i < TN; ++i)
-                    if (i * WN + wn < tiles_n) fz[i] = read_transposed<T, false>(z_lds, PN, c * KC, i * WN + wn, lane);
+                for (int i = 0; i < TN; ++i) {
+                    const int t = i * WN + wn;
+                    fz[i] = read_transposed<T, false>(z_lds, PN, c * KC, t < NT ? t : NT - 1, lane);
+                }
 #pragma unroll
-                for (int j = 0; j < TK; ++j)
-                    if (j * WK + wk < tiles_k) fx[j] = read_transposed<T, false>(x_lds, PK, c * KC, j * WK + wk, lane);
+                for (int j = 0; j < TK; ++j) {
+                    const int t = j * WK + wk;
+                    fx[j] = read_transposed<T, false>(x_lds, PK, c * KC, t < KT ? t : KT - 1, lane);
+                }
 #pragma unroll
                 for (int i = 0; i < TN; ++i) {
-                    if (i * WN + wn >= tiles_n) break;
 #pragma unroll
-                    for (int j = 0; j < TK; ++j) {
-                        if (j * WK + wk >= tiles_k) break;
-                        acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
-                    }
-                    if (wk == 0) acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
+                    for (int j = 0; j < TK; ++j) acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
+                    acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
                 }
             }
         }
