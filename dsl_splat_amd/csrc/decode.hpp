@@ -398,9 +398,10 @@ GS3D_DEV u32x4 finish_row_q8(Q8Raw raw, int at, int channels, bool inside = fals
     const int over = at + E - channels;
     if (!inside && (WIDE || channels >= E) && over > 0) raw.codes = over >= E ? 0u : raw.codes >> (8 * over);
     const float scale = q8_scale(raw.scale);
+    const uint32_t words[2] = {(uint32_t)raw.codes, (uint32_t)(raw.codes >> 32)};
     float v[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = (float)(int)(int8_t)(raw.codes >> (8 * i)) * scale;
+    for (int i = 0; i < E; ++i) v[i] = (float)(int)(int8_t)(words[i / 4] >> (8 * (i & 3))) * scale;
     if (!inside && over > 0) {
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] = at + i < channels ? v[i] : 0.0f;

@@ -78,11 +78,12 @@ GS3D_DEV void merge_moments(float& n, float& mean, float& m2, float nb, float mb
     n = total;
 }
 
-template <class T>
+template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void norm_statistics_kernel(NormShape s, Rows a, float2* __restrict__ part) {
     constexpr int E = VEC<T>;
     constexpr int U = 4;  // pixels whose loads are in flight together
     const NormThread t = norm_thread<E>(s.channels);
+    const bool inside = s.channels % E == 0;  // every vector is whole
     const int64_t begin = blockIdx.x * s.strip_rows, base = blockIdx.y * s.pixels;
     const int64_t end = begin + s.strip_rows < s.pixels ? begin + s.strip_rows : s.pixels;
     float mean[E], m2[E], n = 0.0f;
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(256) void norm_statistics_kernel(NormShape s, Rows 
     for (int i = 0; i < E; ++i) mean[i] = m2[i] = 0.0f;
     if (t.live) {
         for (int64_t p = begin + t.slot; p < end; p += U * t.slots) {
-            RowRaw<T, false> raw[U];
+            RowRaw<T, false, WIDE> raw[U];
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 const int64_t row = p + k * t.slots;
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(256) void norm_statistics_kernel(NormShape s, Rows 
             for (int k = 0; k < U; ++k) {
                 if (p + k * t.slots >= end) break;
                 float v[E];
-                unpack<T>(raw[k].finish(a, t.at), v);
+                unpack<T>(raw[k].finish_in(a, inside, t.at), v);
                 n += 1.0f;
                 const float share = __builtin_amdgcn_rcpf(n);
 #pragma unroll
@@ -182,30 +183,32 @@ __global__ __launch_bounds__(1024) void norm_merge_kernel(NormShape s, const flo
 
 // KEEP: x is also written in 8 bits as it is read; whole blocks of 32 channels
 // then, so that a block lies in neighbouring lanes.
-template <class T, bool KEEP>
+template <class T, bool KEEP, bool WIDE>
 __global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, Rows a, NormParams p, T* __restrict__ y,
                                                          int8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     constexpr int E = VEC<T>;
     constexpr int U = 4;
     const NormThread t = norm_thread<E>(s.channels);
+    const bool inside = s.channels % E == 0;  // every vector is whole
     if (!t.live) return;
     const int64_t begin = blockIdx.x * s.strip_rows, base = blockIdx.y * s.pixels;
     const int64_t end = begin + s.strip_rows < s.pixels ? begin + s.strip_rows : s.pixels;
     float mean[E], rstd[E], scale[E], beta[E];
     norm_constants<T, E>(s, p, blockIdx.y, t.at, mean, rstd, scale, beta);
-    for (int64_t row = begin + t.slot; row < end; row += U * t.slots) {
-        RowRaw<T, false> raw[U];
+    // Backwards: what the first pass read last is still in the cache.
+    for (int64_t row = end - 1 - t.slot; row >= begin; row -= U * t.slots) {
+        RowRaw<T, false, WIDE> raw[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-            const int64_t at = row + k * t.slots;
-            raw[k].issue(a, base + (at < end ? at : row), t.at);
+            const int64_t at = row - k * t.slots;
+            raw[k].issue(a, base + (at >= begin ? at : row), t.at);
         }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-            const int64_t at = row + k * t.slots;
-            if (at >= end) break;
+            const int64_t at = row - k * t.slots;
+            if (at < begin) break;
             float v[E];
-            unpack<T>(raw[k].finish(a, t.at), v);
+            unpack<T>(raw[k].finish_in(a, inside, t.at), v);
             if constexpr (KEEP) q8_keep<T>(v, codes, scales, base + at, t.at, s.channels, true);
 #pragma unroll
             for (int i = 0; i < E; ++i) v[i] = __builtin_fmaf(v[i] - mean[i], scale[i], beta[i]);
@@ -215,35 +218,36 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, Rows a, No
     }
 }
 
-template <class T, bool Q8>
-__global__ __launch_bounds__(256) void norm_sums_kernel(NormShape s, Rows a, NormParams p, const T* __restrict__ dy,
+template <class T, bool Q8, bool WIDE>
+__global__ __launch_bounds__(256, 4) void norm_sums_kernel(NormShape s, Rows a, NormParams p, const T* __restrict__ dy,
                                                         int64_t ldy, float2* __restrict__ part) {
     constexpr int E = VEC<T>;
     constexpr int U = 2;
     const NormThread t = norm_thread<E>(s.channels);
+    const bool inside = s.channels % E == 0;  // every vector is whole
     const int64_t begin = blockIdx.x * s.strip_rows, base = blockIdx.y * s.pixels;
     const int64_t end = begin + s.strip_rows < s.pixels ? begin + s.strip_rows : s.pixels;
-    float s1[E], s2[E], rstd[E];
+    float s1[E], s2[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) s1[i] = s2[i] = rstd[i] = 0.0f;
+    for (int i = 0; i < E; ++i) s1[i] = s2[i] = 0.0f;
     if (t.live) {
-        float mean[E], scale[E], beta[E];
+        float mean[E], rstd[E], scale[E], beta[E];
         norm_constants<T, E>(s, p, blockIdx.y, t.at, mean, rstd, scale, beta);
         for (int64_t row = begin + t.slot; row < end; row += U * t.slots) {
-            RowRaw<T, Q8> raw[U];
+            RowRaw<T, Q8, WIDE> raw[U];
             u32x4 up[U];
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 const int64_t r = row + k * t.slots, at = base + (r < end ? r : row);
                 raw[k].issue(a, at, t.at);
-                up[k] = issue_row(dy + at * ldy, t.at, s.channels);
+                up[k] = issue_row<T, WIDE>(dy + at * ldy, t.at, s.channels);
             }
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 if (row + k * t.slots >= end) break;
                 float v[E], u[E], g[E];
-                unpack<T>(raw[k].finish(a, t.at), v);
-                unpack<T>(finish_row<T>(up[k], t.at, s.channels), g);
+                unpack<T>(raw[k].finish_in(a, inside, t.at), v);
+                unpack<T>(inside ? up[k] : finish_row<T, WIDE>(up[k], t.at, s.channels), g);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     v[i] -= mean[i];
@@ -277,7 +281,10 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(NormShape s, Rows a, Nor
         float2* out = part + ((int64_t)blockIdx.y * s.strips + blockIdx.x) * s.channels + t.at;
 #pragma unroll
         for (int i = 0; i < E; ++i)
-            if (t.at + i < s.channels) out[i] = float2{s1[i], s2[i] * rstd[i]};
+            if (t.at + i < s.channels) {
+                const int group = (t.at + i) / (s.channels / s.groups);
+                out[i] = float2{s1[i], s2[i] * p.stats[(int64_t)blockIdx.y * s.groups + group].y};
+            }
     }
 }
 
@@ -348,13 +355,14 @@ __global__ __launch_bounds__(256) void norm_params_kernel(int images, int channe
     if (dgamma) dgamma[c] = (T)a2;
 }
 
-template <class T, bool Q8>
-__global__ __launch_bounds__(256) void norm_grad_kernel(NormShape s, Rows a, NormParams p, const T* __restrict__ dy,
+template <class T, bool Q8, bool WIDE>
+__global__ __launch_bounds__(256, 4) void norm_grad_kernel(NormShape s, Rows a, NormParams p, const T* __restrict__ dy,
                                                         int64_t ldy, const float2* __restrict__ pulls,
                                                         T* __restrict__ dx) {
     constexpr int E = VEC<T>;
     constexpr int U = 2;
     const NormThread t = norm_thread<E>(s.channels);
+    const bool inside = s.channels % E == 0;  // every vector is whole
     if (!t.live) return;
     const int64_t begin = blockIdx.x * s.strip_rows, base = blockIdx.y * s.pixels;
     const int64_t end = begin + s.strip_rows < s.pixels ? begin + s.strip_rows : s.pixels;
@@ -370,22 +378,22 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormShape s, Rows a, Nor
         level[i] = rstd * pull.x;
         along[i] = rstd * rstd * pull.y;
     }
-    for (int64_t row = begin + t.slot; row < end; row += U * t.slots) {
-        RowRaw<T, Q8> raw[U];
+    for (int64_t row = end - 1 - t.slot; row >= begin; row -= U * t.slots) {  // backwards, as in norm_apply_kernel
+        RowRaw<T, Q8, WIDE> raw[U];
         u32x4 up[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-            const int64_t r = row + k * t.slots, at = base + (r < end ? r : row);
+            const int64_t r = row - k * t.slots, at = base + (r >= begin ? r : row);
             raw[k].issue(a, at, t.at);
-            up[k] = issue_row(dy + at * ldy, t.at, s.channels);
+            up[k] = issue_row<T, WIDE>(dy + at * ldy, t.at, s.channels);
         }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-            const int64_t at = row + k * t.slots;
-            if (at >= end) break;
+            const int64_t at = row - k * t.slots;
+            if (at < begin) break;
             float v[E], u[E], g[E];
-            unpack<T>(raw[k].finish(a, t.at), v);
-            unpack<T>(finish_row<T>(up[k], t.at, s.channels), g);
+            unpack<T>(raw[k].finish_in(a, inside, t.at), v);
+            unpack<T>(inside ? up[k] : finish_row<T, WIDE>(up[k], t.at, s.channels), g);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 v[i] -= mean[i];
@@ -440,22 +448,30 @@ static int norm_fwd(const gs3d_group_norm_args& g, void* scratch, hipStream_t st
     float2* part = static_cast<float2*>(scratch);
     float2* stats = reinterpret_cast<float2*>(g.statistics);
     const dim3 grid = norm_grid(s, g.dtype);
-    hipLaunchKernelGGL(norm_statistics_kernel<T>, grid, dim3(256), 0, stream, s, a, part);
+    const bool wide = g.channels >= VEC<T>;
+    if (wide) hipLaunchKernelGGL((norm_statistics_kernel<T, true>), grid, dim3(256), 0, stream, s, a, part);
+    else hipLaunchKernelGGL((norm_statistics_kernel<T, false>), grid, dim3(256), 0, stream, s, a, part);
     hipLaunchKernelGGL(norm_merge_kernel, dim3(s.groups, s.images), dim3(1024), 0, stream, s, part, stats);
     const NormParams p{g.weight, g.bias, stats};
     T* y = static_cast<T*>(g.y);
     if (g.codes && g.channels % Q8_BLOCK == 0) {
-        hipLaunchKernelGGL((norm_apply_kernel<T, true>), grid, dim3(256), 0, stream, s, a, p, y, g.codes, g.scales);
+        hipLaunchKernelGGL((norm_apply_kernel<T, true, true>), grid, dim3(256), 0, stream, s, a, p, y, g.codes,
+                           g.scales);
     } else {
         if (g.codes)
             quantize_rows(g.x, g.x_stride, g.images * g.pixels, g.channels, g.dtype, g.codes, g.scales, stream);
-        hipLaunchKernelGGL((norm_apply_kernel<T, false>), grid, dim3(256), 0, stream, s, a, p, y, nullptr, nullptr);
+        if (wide)
+            hipLaunchKernelGGL((norm_apply_kernel<T, false, true>), grid, dim3(256), 0, stream, s, a, p, y, nullptr,
+                               nullptr);
+        else
+            hipLaunchKernelGGL((norm_apply_kernel<T, false, false>), grid, dim3(256), 0, stream, s, a, p, y, nullptr,
+                               nullptr);
     }
     return launch_status("gs3d_group_norm_fwd");
 }
 
-template <class T, bool Q8>
-static int norm_bwd(const gs3d_group_norm_bwd_args& g, char* scratch, hipStream_t stream) {
+template <class T, bool Q8, bool WIDE>
+static int norm_bwd_as(const gs3d_group_norm_bwd_args& g, char* scratch, hipStream_t stream) {
     NormShape s = norm_shape(g.images, g.pixels, g.channels, g.groups, g.dtype);
     s.act = g.activation;
     const Rows a{g.x, g.x_stride, {g.codes, g.scales, g.channels}, g.channels};
@@ -466,16 +482,22 @@ static int norm_bwd(const gs3d_group_norm_bwd_args& g, char* scratch, hipStream_
     const T* dy = static_cast<const T*>(g.upstream);
     const T* gamma = static_cast<const T*>(g.weight);
     const dim3 grid = norm_grid(s, g.dtype);
-    hipLaunchKernelGGL((norm_sums_kernel<T, Q8>), grid, dim3(256), 0, stream, s, a, p, dy, g.upstream_stride, part);
+    hipLaunchKernelGGL((norm_sums_kernel<T, Q8, WIDE>), grid, dim3(256), 0, stream, s, a, p, dy, g.upstream_stride,
+                       part);
     hipLaunchKernelGGL(norm_totals_kernel<T>, dim3(s.groups, s.images), dim3(1024), 0, stream, s, gamma, part, sums,
                        pulls);
     if (g.grad_x)
-        hipLaunchKernelGGL((norm_grad_kernel<T, Q8>), grid, dim3(256), 0, stream, s, a, p, dy, g.upstream_stride,
+        hipLaunchKernelGGL((norm_grad_kernel<T, Q8, WIDE>), grid, dim3(256), 0, stream, s, a, p, dy, g.upstream_stride,
                            pulls, static_cast<T*>(g.grad_x));
     if (g.grad_weight || g.grad_bias)
-        hipLaunchKernelGGL(norm_params_kernel<T>, dim3(blocks_for(s.channels, 256)), dim3(256), 0, stream, s.images,
+        hipLaunchKernelGGL(norm_params_kernel<T>, dim3(blocks_for(s.channels, 256)), dim3(256), 0, stream, g.images,
                            s.channels, sums, static_cast<T*>(g.grad_weight), static_cast<T*>(g.grad_bias));
     return launch_status("gs3d_group_norm_bwd");
+}
+template <class T, bool Q8>
+static int norm_bwd(const gs3d_group_norm_bwd_args& g, char* scratch, hipStream_t stream) {
+    return g.channels >= VEC<T> ? norm_bwd_as<T, Q8, true>(g, scratch, stream)
+                                : norm_bwd_as<T, Q8, false>(g, scratch, stream);
 }
 
 static bool norm_sizes_ok(int32_t images, int64_t pixels, int32_t channels, int32_t groups, int dtype, int activation) {

@@ -28,13 +28,22 @@ constexpr int fused_waves() {
     return 4;
 }
 
-// A block of 8 wavefronts takes 64 rows at a time, KCH chunks of K and NCH of
-// N wide, over a range of rows of its own.
+// Strips of 16 rows that a wavefront takes at a time: two where two blocks of
+// that size still share a compute unit's LDS.
+template <class T, int KCH, int NCH>
+constexpr int fused_strips() {
+    const int pad = sizeof(T) == 4 ? 1 : 2;
+    const int w = NCH * CHUNK<T> * (KCH * 4 + pad) * 16 + NCH * CHUNK<T> * 4;
+    return w + 128 * ((KCH + NCH) * 4 + 2 * pad) * 16 <= 81920 ? 2 : 1;
+}
+
+// A block of 8 wavefronts takes ROWS = 64 or 128 rows at a time, KCH chunks of
+// K and NCH of N wide, over a range of rows of its own.
 //
 // x and dy go to LDS as they lie in memory, row by row (whole lines an
-// instruction), the next 64 rows on their way while these are worked on.
+// instruction), the next rows on their way while these are worked on.
 //
-// First dz.  Wavefronts s and s + 4 take rows 16 s..16 s + 15, every other
+// First dz.  Wavefronts s and s + 4 take strip s of 16 rows (and s + 4), every other
 // chunk of N each: lane l has row l % 16 and the elements from VEC (l / 16) on
 // of a chunk, of x as of dy.  With W's rows as the first operand, z comes out
 // with that row in that lane and, W's rows dealt out as tile_column says, with
@@ -66,14 +75,15 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
     // Vectors are dealt to threads by powers of two a row; a row of 6 or 7
     // chunks leaves some without.
     constexpr int DN = NCH > 4 ? 32 : VN;
-    constexpr int LK = (64 * VK + 511) / 512, LN = (64 * DN + 511) / 512;
+    constexpr int RB = fused_strips<T, KCH, NCH>(), ROWS = 64 * RB;
+    constexpr int LK = (ROWS * VK + 511) / 512, LN = (ROWS * DN + 511) / 512;
     __shared__ u32x4 w_lds[NCH * KC * PK];
-    __shared__ u32x4 x_lds[64 * PK];
-    __shared__ u32x4 z_lds[64 * PN];
+    __shared__ u32x4 x_lds[ROWS * PK];
+    __shared__ u32x4 z_lds[ROWS * PN];
     __shared__ f32x4 bias_lds[NCH * KC / 4];
 
     const int tid = threadIdx.x, wave = wave_id();
-    const int strip = (wave & 3) * 16, half = wave >> 2;
+    const int half = wave >> 2;
     const int wn = wave / WK, wk = wave % WK;
     const int64_t begin = blockIdx.x * a.rows_per_block;
     const int64_t end = begin + a.rows_per_block < a.rows ? begin + a.rows_per_block : a.rows;
@@ -120,18 +130,18 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
     // Rows past the end add nothing, whatever the last row holds.
     auto fill = [&](int64_t m0) {
         const u32x4 zero = {0u, 0u, 0u, 0u};
-        const bool whole = m0 + 64 <= end;
+        const bool whole = m0 + ROWS <= end;
 #pragma unroll
         for (int i = 0; i < LK; ++i) {
             const int u = i * 512 + tid;
-            if (64 * VK % 512 != 0 && u >= 64 * VK) break;
+            if (ROWS * VK % 512 != 0 && u >= ROWS * VK) break;
             u32x4 v = xr[i].finish_in(a.x, VK * E <= a.K, u % VK * E);
             x_lds[u / VK * PK + u % VK] = whole || m0 + u / VK < end ? v : zero;
         }
 #pragma unroll
         for (int i = 0; i < LN; ++i) {
             const int u = i * 512 + tid;
-            if (64 * DN % 512 != 0 && u >= 64 * DN) break;
+            if (ROWS * DN % 512 != 0 && u >= ROWS * DN) break;
             u32x4 v = yr[i];
             if (VN * E > a.N) v = finish_row<T, WIDE>(v, u % DN * E, a.N);
             if (DN == VN || u % DN < VN) z_lds[u / DN * PN + u % DN] = whole || m0 + u / DN < end ? v : zero;
@@ -139,9 +149,9 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
     };
 
     if (begin < end) load(begin);
-    for (int64_t m0 = begin; m0 < end; m0 += 64) {
+    for (int64_t m0 = begin; m0 < end; m0 += ROWS) {
         fill(m0);
-        if (m0 + 64 < end) load(m0 + 64);
+        if (m0 + ROWS < end) load(m0 + ROWS);
         __syncthreads();
         // Opaque in every round: the tiles' addresses, all of them loop
         // invariant, would otherwise fill the registers.
@@ -149,67 +159,77 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
         asm volatile("" : "+v"(lane));
         const int r = lane & 15, q = lane >> 4;
         if (a.act != GS3D_ACT_NONE) {
-            u32x4 xf[KCH];
 #pragma unroll
-            for (int c = 0; c < KCH; ++c) xf[c] = x_lds[(strip + r) * PK + c * 4 + q];
+            for (int b = 0; b < RB; ++b) {
+                const int strip = (b * 4 + (wave & 3)) * 16;
+                u32x4 xf[KCH];
 #pragma unroll
-            for (int gi = 0; gi < HN; ++gi) {
-                const int g = 2 * gi + half;
-                if (g >= NCH || (SKIP && g * KC >= a.N)) break;
-                f32x4 z[TG];
+                for (int c = 0; c < KCH; ++c) xf[c] = x_lds[(strip + r) * PK + c * 4 + q];
 #pragma unroll
-                for (int t = 0; t < TG; ++t) z[t] = bias_lds[g * 4 * TG + q * TG + t];
+                for (int gi = 0; gi < HN; ++gi) {
+                    const int g = NCH == 1 ? 0 : 2 * gi + half;
+                    if (NCH == 1 && half != (RB == 2 ? b : 0)) break;  // one chunk: a strip each
+                    if (g >= NCH || (SKIP && g * KC >= a.N)) break;
+                    f32x4 z[TG];
 #pragma unroll
-                for (int c = 0; c < KCH; ++c)
+                    for (int t = 0; t < TG; ++t) z[t] = bias_lds[g * 4 * TG + q * TG + t];
 #pragma unroll
-                    for (int t = 0; t < TG; ++t)
-                        z[t] = multiply_chunk<T>(w_lds[tile_column<T>(g * TG + t, r) * PK + c * 4 + q], xf[c], z[t],
-                                                 a.K - c * KC);
-                settle(z);
-                u32x4& slot = z_lds[(strip + r) * PN + g * 4 + q];
-                float arg[E], grad[E];
-                unpack<T>(slot, grad);
+                    for (int c = 0; c < KCH; ++c)
 #pragma unroll
-                for (int i = 0; i < E; ++i) arg[i] = z[i / 4][i & 3];
-                pull_back(grad, arg, a.act);
-                slot = pack<T>(grad);
+                        for (int t = 0; t < TG; ++t)
+                            z[t] = multiply_chunk<T>(w_lds[tile_column<T>(g * TG + t, r) * PK + c * 4 + q], xf[c], z[t],
+                                                     a.K - c * KC);
+                    settle(z);
+                    u32x4& slot = z_lds[(strip + r) * PN + g * 4 + q];
+                    float arg[E], grad[E];
+                    unpack<T>(slot, grad);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) arg[i] = z[i / 4][i & 3];
+                    pull_back(grad, arg, a.act);
+                    slot = pack<T>(grad);
+                }
             }
             __syncthreads();
         }
         if (dx) {
-            const int64_t m = m0 + strip + r;
-            // Float's twice as many vectors are read where they are used.
-            u32x4 dz[SKIP ? 1 : NCH];
-            if constexpr (!SKIP) {
 #pragma unroll
-                for (int g = 0; g < NCH; ++g) dz[g] = z_lds[(strip + r) * PN + g * 4 + q];
-            }
+            for (int b = 0; b < RB; ++b) {
+                const int strip = (b * 4 + (wave & 3)) * 16;
+                const int64_t m = m0 + strip + r;
+                // Float's twice as many vectors are read where they are used.
+                u32x4 dz[SKIP ? 1 : NCH];
+                if constexpr (!SKIP) {
 #pragma unroll
-            for (int ci = 0; ci < HK; ++ci) {
-                const int c = 2 * ci + half;
-                if (c >= KCH || (SKIP && c * KC >= a.K)) break;
-                f32x4 out[TG];
-#pragma unroll
-                for (int t = 0; t < TG; ++t) out[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int g = 0; g < NCH; ++g) {
-                    if (SKIP && g * KC >= a.N) break;
-                    if constexpr (SKIP) dz[0] = z_lds[(strip + r) * PN + g * 4 + q];
-#pragma unroll
-                    for (int t = 0; t < TG; ++t)
-                        out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, c * TG + t, lane),
-                                                   dz[SKIP ? 0 : g], out[t], a.N - g * KC);
+                    for (int g = 0; g < NCH; ++g) dz[g] = z_lds[(strip + r) * PN + g * 4 + q];
                 }
-                settle(out);
-                float v[E];
 #pragma unroll
-                for (int i = 0; i < E; ++i) v[i] = out[i / 4][i & 3];
-                if (m < end) store_chunk(dx + m * a.K, c * KC, c * KC + q * E, a.K, pack<T>(v));
+                for (int ci = 0; ci < HK; ++ci) {
+                    const int c = KCH == 1 ? 0 : 2 * ci + half;
+                    if (KCH == 1 && half != (RB == 2 ? b : 0)) break;
+                    if (c >= KCH || (SKIP && c * KC >= a.K)) break;
+                    f32x4 out[TG];
+#pragma unroll
+                    for (int t = 0; t < TG; ++t) out[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int g = 0; g < NCH; ++g) {
+                        if (SKIP && g * KC >= a.N) break;
+                        if constexpr (SKIP) dz[0] = z_lds[(strip + r) * PN + g * 4 + q];
+#pragma unroll
+                        for (int t = 0; t < TG; ++t)
+                            out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, c * TG + t, lane),
+                                                       dz[SKIP ? 0 : g], out[t], a.N - g * KC);
+                    }
+                    settle(out);
+                    float v[E];
+#pragma unroll
+                    for (int i = 0; i < E; ++i) v[i] = out[i / 4][i & 3];
+                    if (m < end) store_chunk(dx + m * a.K, c * KC, c * KC + q * E, a.K, pack<T>(v));
+                }
             }
         }
         if (a.part) {
 #pragma unroll
-            for (int c = 0; c < 64 / KC; ++c) {
+            for (int c = 0; c < ROWS / KC; ++c) {
                 // Where the tiles do not share out evenly the last one is taken
                 // again, and not stored.
                 u32x4 fz[TN], fx[TK];
