@@ -454,6 +454,31 @@ GS3D_DEV void store_chunk(T* row, int first, int at, int count, u32x4 raw) {
 GS3D_DEV int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // ---------------------------------------------------------------------------
+// A gradient dz = dy act'(z) is computed in 32 bits and then an operand of two
+// matrix products.  Rounded once to 16 bits it makes the error of dx 1.33 to
+// 1.41 times, that of dW and db 1.34 to 1.53 times what rounding the results
+// alone gives (relu, silu and gelu, 100000 rows).  dW, which a training step
+// adds up over many calls, takes dz as two 16-bit values, high and low, and is
+// then as exact as its own rounding; dx takes the high one.  At 128 to 128
+// channels of bfloat16 and 1.92 M rows: one value 387 us, the low one in dW
+// 502 us, in dx as well 556 us.  Float, and dy itself where there is no
+// activation, are one value.
+// ---------------------------------------------------------------------------
+template <class T>
+constexpr bool SPLIT = sizeof(T) == 2;
+
+// The vector's high halves; v keeps what they leave, nothing beside an infinity.
+template <class T>
+GS3D_DEV u32x4 take_high(float (&v)[VEC<T>]) {
+    const u32x4 high = pack<T>(v);
+    float h[VEC<T>];
+    unpack<T>(high, h);
+#pragma unroll
+    for (int i = 0; i < VEC<T>; ++i) v[i] = __builtin_isinf(h[i]) ? 0.0f : v[i] - h[i];
+    return high;
+}
+
+// ---------------------------------------------------------------------------
 // Matrix fragments.  A fragment is 16 bytes a lane: lane l holds row l % 16
 // and, in the contracted dimension, the VEC<T> elements from VEC<T> * (l / 16)
 // on; 64 lanes hold 16 rows x CHUNK<T> elements.  multiply() adds

@@ -31,6 +31,7 @@ struct LinearRows {
     const void* other;   // EPI 1: dy; EPI 2: residual
     int64_t ldo;
     void* y;             // rows x N
+    void* low;           // EPI 1 of 16-bit types: what y leaves of dz, rows x N
     int64_t rows;
     int K, N, act, n_tiles, strips;
     int8_t* keep_codes;  // where the rows of x are kept in 8 bits, or NULL
@@ -45,14 +46,20 @@ GS3D_DEV void xcd_block(const LinearRows& a, int64_t& row_block, int& n_tile) {
     n_tile = (int)(local % a.n_tiles);
 }
 
+template <class T, int EPI>
+constexpr bool KEEPS_LOW = EPI == 1 && SPLIT<T>;
+
 // The end of a product for one lane's vector of E neighbouring outputs.
 template <class T, int EPI, int E>
-GS3D_DEV u32x4 linear_end(const LinearRows& a, float (&z)[E], u32x4 raw_other) {
+GS3D_DEV u32x4 linear_end(const LinearRows& a, float (&z)[E], u32x4 raw_other, u32x4& low) {
     float o[E];
     if constexpr (EPI != 0) unpack<T>(raw_other, o);
     if constexpr (EPI == 1) {
         pull_back(o, z, a.act);
-        return pack<T>(o);
+        if constexpr (!SPLIT<T>) return pack<T>(o);
+        const u32x4 high = take_high<T>(o);
+        low = pack<T>(o);
+        return high;
     } else {
         activate(z, a.act);
         if constexpr (EPI == 2) {
@@ -94,10 +101,11 @@ GS3D_DEV void store_strip(const u32x4* strip, T* y, int64_t first, int64_t end, 
 }
 
 // Wavefronts a SIMD that the stream kernel's registers leave room for.
-template <class T, bool Q8, int EPI, int KCH, int NT>
+template <class T, bool Q8, int EPI, int KCH, int NT, bool WIDE>
 constexpr int stream_waves() {
     const int wide = sizeof(T) == 4 ? 2 : 1;  // float holds twice the vectors
-    const int vectors = wide * (2 * KCH + (EPI != 0 ? NT / 2 : 0));
+    const int vectors =
+        wide * (2 * KCH + (EPI != 0 ? NT / 2 : 0)) + (KEEPS_LOW<T, EPI> ? NT / 2 + 1 : 0) + (WIDE ? 0 : 3);
     return vectors <= 4 ? 6 : vectors <= 8 ? 5 : vectors <= 12 ? 4 : vectors <= 16 ? 3 : 2;
 }
 
@@ -119,7 +127,7 @@ constexpr int stream_waves() {
 // first, and whole strips store without a branch: the wait for a load then
 // leaves the stores after it in flight.
 template <class T, bool Q8, int EPI, int KCH, int NT, bool WIDE>
-__global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void linear_stream_kernel(LinearRows a) {
+__global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT, WIDE>())) void linear_stream_kernel(LinearRows a) {
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
     constexpr int TG = KC / 16;  // tiles of a lane's 16-byte output vector
@@ -210,6 +218,7 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
             }
             wave_fence();
         }
+        u32x4 low[G];
         // The weights stay in LDS: hoisted out of the loop they would take
         // every register (128 at 4 chunks x 8 tiles).
         int at_w = lane;
@@ -232,13 +241,24 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT>())) void li
             u32x4& slot = mine[r * PO + g * 4 + q];
             u32x4 raw = {0u, 0u, 0u, 0u};
             if constexpr (EPI != 0) raw = slot;
-            raw = linear_end<T, EPI, E>(a, z, raw);
+            raw = linear_end<T, EPI, E>(a, z, raw, low[g]);
             const int64_t m = m0 + r;
             if (staged) slot = raw;
-            else if (whole.value || m < end) store_chunk(y + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
+            else if (whole.value || m < end) {
+                store_chunk(y + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
+                if constexpr (KEEPS_LOW<T, EPI>)
+                    store_chunk(static_cast<T*>(a.low) + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, low[g]);
+            }
         }
         if (staged) store_strip<T, VP, PO>(mine, y, m0, end, n0, a.N, lane, whole);
         else wave_fence();
+        if constexpr (KEEPS_LOW<T, EPI>) {
+            if (staged) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) mine[r * PO + g * 4 + q] = low[g];
+                store_strip<T, VP, PO>(mine, static_cast<T*>(a.low), m0, end, n0, a.N, lane, whole);
+            }
+        }
     };
     for (; m0 + 16 <= end; m0 += 64) strip(m0, Flag<true>{});
     if (m0 < end) strip(m0, Flag<false>{});
@@ -353,7 +373,7 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     for (int s = 0; s < RS; ++s) {
         const int64_t m = first + wave * (16 * RS) + 16 * s + r;
         const int64_t at_row = m < a.rows ? m : a.rows - 1;
-        u32x4 o[G];
+        u32x4 o[G], low[G];
         if constexpr (EPI != 0) {
 #pragma unroll
             for (int g = 0; g < G; ++g) o[g] = issue_row<T, WIDE>(other + at_row * a.ldo, n0 + g * KC + q * E, a.N);
@@ -366,13 +386,25 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
             for (int i = 0; i < E; ++i) z[i] = acc[s][g * TG + i / 4][i & 3] + bias_lds[at + i];
             u32x4 raw = {0u, 0u, 0u, 0u};
             if constexpr (EPI != 0) raw = finish_chunk<T, WIDE>(o[g], n0 + g * KC, n0 + at, a.N);
-            raw = linear_end<T, EPI, E>(a, z, raw);
+            raw = linear_end<T, EPI, E>(a, z, raw, low[g]);
             if (staged) strip[r * PO + g * 4 + q] = raw;
-            else if (m < a.rows) store_chunk(y + m * a.N, n0 + g * KC, n0 + at, a.N, raw);
+            else if (m < a.rows) {
+                store_chunk(y + m * a.N, n0 + g * KC, n0 + at, a.N, raw);
+                if constexpr (KEEPS_LOW<T, EPI>)
+                    store_chunk(static_cast<T*>(a.low) + m * a.N, n0 + g * KC, n0 + at, a.N, low[g]);
+            }
         }
+        auto put = [&](T* to) {
+            if (m - r + 16 <= a.rows) store_strip<T, VP, PO>(strip, to, m - r, a.rows, n0, a.N, lane, Flag<true>{});
+            else store_strip<T, VP, PO>(strip, to, m - r, a.rows, n0, a.N, lane, Flag<false>{});
+        };
         if (staged) {
-            if (m - r + 16 <= a.rows) store_strip<T, VP, PO>(strip, y, m - r, a.rows, n0, a.N, lane, Flag<true>{});
-            else store_strip<T, VP, PO>(strip, y, m - r, a.rows, n0, a.N, lane, Flag<false>{});
+            put(y);
+            if constexpr (KEEPS_LOW<T, EPI>) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) strip[r * PO + g * 4 + q] = low[g];
+                put(static_cast<T*>(a.low));
+            }
         }
     }
 }
@@ -519,6 +551,7 @@ void linear_tile_kernel(LinearRows a) {
                 }
                 wave_fence();
             }
+            u32x4 low[G];
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 float z[E];
@@ -527,13 +560,23 @@ void linear_tile_kernel(LinearRows a) {
                 u32x4& slot = mine[r * PO + g * 4 + q];
                 u32x4 raw = {0u, 0u, 0u, 0u};
                 if constexpr (EPI != 0) raw = slot;
-                raw = linear_end<T, EPI, E>(a, z, raw);
+                raw = linear_end<T, EPI, E>(a, z, raw, low[g]);
                 if (staged) slot = raw;
-                else if (whole.value || m < a.rows)
+                else if (whole.value || m < a.rows) {
                     store_chunk(y + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
+                    if constexpr (KEEPS_LOW<T, EPI>)
+                        store_chunk(static_cast<T*>(a.low) + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, low[g]);
+                }
             }
             if (staged) store_strip<T, VP, PO>(mine, y, m0, a.rows, n0, a.N, lane, whole);
             else wave_fence();
+            if constexpr (KEEPS_LOW<T, EPI>) {
+                if (staged) {
+#pragma unroll
+                    for (int g = 0; g < G; ++g) mine[r * PO + g * 4 + q] = low[g];
+                    store_strip<T, VP, PO>(mine, static_cast<T*>(a.low), m0, a.rows, n0, a.N, lane, whole);
+                }
+            }
         };
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -561,6 +604,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ w,
 struct LinearGradW {
     Rows x;
     const void* dz;
+    const void* low;  // what dz leaves, rows x N, or NULL
     int64_t ldz;
     int64_t rows, rows_per_split;
     int N, n_tiles, k_tiles;
@@ -572,7 +616,7 @@ struct LinearGradW {
 // The contracted dimension is the row, the slow one of both operands: they go
 // to LDS as they are, row by row, and are read transposed.  2 x 2 wavefronts
 // multiply 16 A x 16 B columns each.
-template <class T, bool Q8, int A, int B>
+template <class T, bool Q8, int A, int B, int PLANES>
 __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
@@ -581,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
     constexpr int PAD = sizeof(T) == 4 ? 1 : 2;      // spreads rows over the banks
     constexpr int PZ = CZ + PAD, PX = CX + PAD;
     constexpr int LZ = (MR * CZ + 255) / 256, LX = (MR * CX + 255) / 256;
-    __shared__ u32x4 z_lds[MR * PZ];
+    __shared__ u32x4 z_lds[PLANES][MR * PZ];
     __shared__ u32x4 x_lds[MR * PX];
 
     int64_t b = blockIdx.x;
@@ -596,16 +640,17 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
     const int r = lane & 15, q = lane >> 4;
     const int wn = wave >> 1, wk = wave & 1;
     const bool sum_bias = kt == 0 && wk == 0;
-    const T* dz = static_cast<const T*>(a.dz);
+    const T* dz[2] = {static_cast<const T*>(a.dz), static_cast<const T*>(a.low)};
 
-    u32x4 zr[LZ];
+    u32x4 zr[PLANES][LZ];
     RowRaw<T, Q8> xr[LX];
     auto load = [&](int64_t m0) {
 #pragma unroll
         for (int i = 0; i < LZ; ++i) {
             const int u = i * 256 + tid;
             const int64_t m = m0 + u / CZ < end ? m0 + u / CZ : end - 1;
-            zr[i] = issue_row(dz + m * a.ldz, n0 + u % CZ * E, a.N);
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) zr[p][i] = issue_row(dz[p] + m * a.ldz, n0 + u % CZ * E, a.N);
         }
 #pragma unroll
         for (int i = 0; i < LX; ++i) {
@@ -618,9 +663,12 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
 #pragma unroll
         for (int i = 0; i < LZ; ++i) {
             const int u = i * 256 + tid;
-            const u32x4 v = finish_row<T>(zr[i], n0 + u % CZ * E, a.N);
-            if (MR * CZ % 256 == 0 || u < MR * CZ)
-                z_lds[u / CZ * PZ + u % CZ] = m0 + u / CZ < end ? v : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) {
+                const u32x4 v = finish_row<T>(zr[p][i], n0 + u % CZ * E, a.N);
+                if (MR * CZ % 256 == 0 || u < MR * CZ)
+                    z_lds[p][u / CZ * PZ + u % CZ] = m0 + u / CZ < end ? v : u32x4{0u, 0u, 0u, 0u};
+            }
         }
 #pragma unroll
         for (int i = 0; i < LX; ++i) {
@@ -651,19 +699,23 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
         if (m0 + MR < end) load(m0 + MR);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            u32x4 fz[A], fx[B];
-#pragma unroll
-            for (int i = 0; i < A; ++i) fz[i] = read_transposed<T, false>(z_lds, PZ, c * KC, wn * A + i, lane);
+            u32x4 fx[B];
 #pragma unroll
             for (int j = 0; j < B; ++j) fx[j] = read_transposed<T, false>(x_lds, PX, c * KC, wk * B + j, lane);
 #pragma unroll
-            for (int i = 0; i < A; ++i)
+            for (int p = 0; p < PLANES; ++p) {
+                u32x4 fz[A];
 #pragma unroll
-                for (int j = 0; j < B; ++j) acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
-            if (sum_bias) {
+                for (int i = 0; i < A; ++i) fz[i] = read_transposed<T, false>(z_lds[p], PZ, c * KC, wn * A + i, lane);
 #pragma unroll
-                for (int i = 0; i < A; ++i) acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
-                settle(acc_b);
+                for (int i = 0; i < A; ++i)
+#pragma unroll
+                    for (int j = 0; j < B; ++j) acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
+                if (sum_bias) {
+#pragma unroll
+                    for (int i = 0; i < A; ++i) acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
+                    settle(acc_b);
+                }
             }
         }
     }
@@ -807,8 +859,14 @@ static void launch_rows(LinearRows a, void* packed, hipStream_t stream) {
 
 template <class T, bool Q8, int A, int B>
 static void launch_gradw_as(const LinearGradW& a, int splits, hipStream_t stream) {
-    hipLaunchKernelGGL((linear_gradw_kernel<T, Q8, A, B>), dim3((unsigned)(a.n_tiles * a.k_tiles * splits)), dim3(256),
-                       0, stream, a);
+    const dim3 grid((unsigned)(a.n_tiles * a.k_tiles * splits));
+    if constexpr (SPLIT<T>) {
+        if (a.low) {
+            hipLaunchKernelGGL((linear_gradw_kernel<T, Q8, A, B, 2>), grid, dim3(256), 0, stream, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((linear_gradw_kernel<T, Q8, A, B, 1>), grid, dim3(256), 0, stream, a);
 }
 template <class T, bool Q8, int A>
 static void launch_gradw_b(const LinearGradW& a, int splits, hipStream_t stream) {
@@ -852,9 +910,9 @@ static BwdPlan bwd_plan(int64_t rows, int K, int N) {
 static size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Scratch of the backward pass: the splits' dW and db; unless it is fused also
-// dz and W^T.
+// dz, in two planes where it is split, and W^T.
 struct BwdScratch {
-    size_t part, dz, wt, total;
+    size_t part, dz, low, wt, total;
 };
 template <class T>
 static BwdScratch bwd_scratch(int64_t rows, int K, int N) {
@@ -862,7 +920,9 @@ static BwdScratch bwd_scratch(int64_t rows, int K, int N) {
     BwdScratch s;
     s.part = 0;
     s.dz = aligned((size_t)p.splits * ((size_t)N * K + N) * 4);
-    s.wt = s.dz + (p.fused ? 0 : aligned((size_t)rows * N * sizeof(T)));
+    const size_t plane = p.fused ? 0 : aligned((size_t)rows * N * sizeof(T));
+    s.low = s.dz + plane;
+    s.wt = s.low + (SPLIT<T> ? plane : 0);
     // W^T as it is, or packed; W packed in its place before.
     const size_t packed = (size_t)(packed_vectors<T>(N, K) > packed_vectors<T>(K, N) ? packed_vectors<T>(N, K)
                                                                                        : packed_vectors<T>(K, N)) * 16;
@@ -901,22 +961,24 @@ static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t 
     const Rows x{seen ? g.x : g.weight, seen ? g.x_stride : 0, {g.codes, g.scales, g.inner}, g.inner};
     const bool params = g.grad_weight || g.grad_bias;
     float* part = reinterpret_cast<float*>(scratch + at.part);
+    int splits = p.splits;
     if (p.fused) {
         if (g.rows > 0 || params) {
             LinearFused a{x, g.weight, g.bias, g.upstream, g.upstream_stride, g.grad_x, params ? part : nullptr,
-                          g.rows, p.rows_per_split, g.inner, g.outer, g.activation};
+                          g.rows, p.rows_per_split, g.inner, g.outer, g.activation, &splits};
             fused_launch<T>(a, Q8, p.splits, stream);
         }
     } else {
-        const void* dz = g.upstream;
+        const void *dz = g.upstream, *low = nullptr;
         int64_t ldz = g.upstream_stride;
         if (g.activation != GS3D_ACT_NONE && g.rows > 0) {
             LinearRows a{};
             a.x = x, a.w = g.weight, a.bias = g.bias, a.other = g.upstream, a.ldo = g.upstream_stride;
-            a.y = scratch + at.dz;
+            a.y = scratch + at.dz, a.low = scratch + at.low;
             a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
             launch_rows<T, Q8, 1, false>(a, scratch + at.wt, stream);
             dz = scratch + at.dz;
+            if (SPLIT<T>) low = scratch + at.low;
             ldz = g.outer;
         }
         if (g.grad_x && g.rows > 0) {
@@ -926,13 +988,13 @@ static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t 
             launch_rows<T, false, 0, true>(a, scratch + at.wt, stream);
         }
         if (params) {
-            LinearGradW a{x, dz, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, part, g.inner};
+            LinearGradW a{x, dz, low, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, part, g.inner};
             launch_gradw<T, Q8>(a, p.splits, stream);
         }
     }
     if (params) {
         const int64_t weights = (int64_t)g.outer * g.inner, count = weights + g.outer;
-        hipLaunchKernelGGL(sum_splits_kernel<T>, dim3(blocks_for(count, 32)), dim3(256), 0, stream, part, p.splits,
+        hipLaunchKernelGGL(sum_splits_kernel<T>, dim3(blocks_for(count, 32)), dim3(256), 0, stream, part, splits,
                            weights, count, static_cast<T*>(g.grad_weight), static_cast<T*>(g.grad_bias));
     }
     return launch_status("gs3d_linear_bwd");

@@ -17,73 +17,75 @@ struct LinearFused {
     float* part;       // blocks x (N K + N): the blocks' shares of dW and db, or NULL
     int64_t rows, rows_per_block;
     int K, N, act;
+    int* blocks;       // host: receives how many blocks were launched
 };
 
-// Wavefronts a SIMD: four where the registers do without scratch memory (128 x
-// 128 of bfloat16 at four: 681 us for the case below).
-template <class T, int KCH, int NCH>
-constexpr int fused_waves() {
-    // Two blocks of float fit where W and both tiles take 80 KB at most.
-    if (sizeof(T) == 4) return (NCH * 16 * (KCH * 4 + 1) + 64 * (KCH + NCH) * 4 + 128) * 16 + NCH * 64 > 81920 ? 2 : 4;
-    return 4;
-}
+// How a backward kernel of KCH x NCH chunks lies on a compute unit: two blocks
+// of 8 wavefronts where their LDS fits, of 128 rows or 64; else one of 16, the
+// weights once for all of them.  Four wavefronts a SIMD either way.
+template <class T, int KCH, int NCH, bool ACT>
+struct FusedShape {
+    static constexpr int PLANES = SPLIT<T> && ACT ? 2 : 1;
+    static constexpr int PAD = sizeof(T) == 4 ? 1 : 2;
+    static constexpr int FIXED = NCH * CHUNK<T> * ((KCH * 4 + PAD) * 16 + 4);
+    static constexpr int ROW = (KCH * 4 + PAD + PLANES * (NCH * 4 + PAD)) * 16;
+    static constexpr bool TWO = FIXED + 64 * ROW <= 81920;
+    static constexpr int WAVES = TWO ? 8 : 16;
+    static constexpr int ROWS = FIXED + 128 * ROW <= (TWO ? 81920 : 163840) ? 128 : 64;
+    static constexpr int STRIPS = ROWS == 128 && WAVES == 16 ? 8 : 4;  // of 16 rows, taken at a time
+    static constexpr int PARTS = WAVES / STRIPS;                       // wavefronts that share a strip
+    static constexpr int RB = ROWS / (16 * STRIPS);
+};
 
-// Strips of 16 rows that a wavefront takes at a time: two where two blocks of
-// that size still share a compute unit's LDS.
-template <class T, int KCH, int NCH>
-constexpr int fused_strips() {
-    const int pad = sizeof(T) == 4 ? 1 : 2;
-    const int w = NCH * CHUNK<T> * (KCH * 4 + pad) * 16 + NCH * CHUNK<T> * 4;
-    return w + 128 * ((KCH + NCH) * 4 + 2 * pad) * 16 <= 81920 ? 2 : 1;
-}
-
-// A block of 8 wavefronts takes ROWS = 64 or 128 rows at a time, KCH chunks of
-// K and NCH of N wide, over a range of rows of its own.
+// A block takes ROWS rows at a time, KCH chunks of K and NCH of N wide, over a
+// range of rows of its own.
 //
 // x and dy go to LDS as they lie in memory, row by row (whole lines an
 // instruction), the next rows on their way while these are worked on.
 //
-// First dz.  Wavefronts s and s + 4 take strip s of 16 rows (and s + 4), every other
-// chunk of N each: lane l has row l % 16 and the elements from VEC (l / 16) on
-// of a chunk, of x as of dy.  With W's rows as the first operand, z comes out
-// with that row in that lane and, W's rows dealt out as tile_column says, with
-// dy's elements beside it, so dz = dy act'(z) takes dy's place vector by
-// vector.
+// First dz.  PARTS wavefronts take a strip of 16 rows, every PARTS-th chunk of
+// N each: lane l has row l % 16 and the elements from VEC (l / 16) on of a
+// chunk, of x as of dy.  With W's rows as the first operand, z comes out with
+// that row in that lane and, W's rows dealt out as tile_column says, with dy's
+// elements beside it, so dz = dy act'(z) takes dy's place vector by vector,
+// its low half in a second plane.
 //
 // Then dx = dz W and dW = dz^T x.  dx takes dz from LDS as it lies and W
-// transposed (W is in LDS once, row by row), every other chunk of K a
+// transposed (W is in LDS once, row by row), every PARTS-th chunk of K a
 // wavefront.  dW contracts over rows: both operands are read transposed, and
-// each wavefront's share of its tiles (4 x 2) stays in its registers over all
-// the block's rows.
+// each wavefront's share of its tiles stays in its registers over all the
+// block's rows.
 //
-// Bytes bound it where K and N are small (x and dy in, dx out).  Two blocks,
-// 16 wavefronts, share a compute unit where their LDS and registers fit, so
-// one block's loads and slopes run under the other's products.
-template <class T, bool Q8, int KCH, int NCH, bool WIDE>
-__global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_fused_kernel(LinearFused a) {
+// Bytes bound it where K and N are small (x and dy in, dx out), the vector
+// units where the slope is dear; four wavefronts a SIMD let one's loads and
+// slopes run under another's products.
+template <class T, bool Q8, int KCH, int NCH, bool WIDE, bool ACT>
+__global__ __launch_bounds__((FusedShape<T, KCH, NCH, ACT>::WAVES * 64), 4) void linear_bwd_fused_kernel(LinearFused a) {
+    using S = FusedShape<T, KCH, NCH, ACT>;
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
     constexpr int TG = KC / 16;  // tiles a chunk
     constexpr int KT = KCH * TG, NT = NCH * TG;
-    constexpr int WN = 4, WK = 2;
+    constexpr int THREADS = S::WAVES * 64, PLANES = S::PLANES, PARTS = S::PARTS;
+    constexpr int WK_MOST = S::WAVES / (NT < 4 ? 2 : 4);  // wavefronts along K and N, none without a tile
+    constexpr int WK = KT < WK_MOST ? KT : WK_MOST, WN = S::WAVES / WK;
     constexpr int TN = (NT + WN - 1) / WN, TK = (KT + WK - 1) / WK;
-    constexpr int HN = (NCH + 1) / 2, HK = (KCH + 1) / 2;
+    constexpr int HN = (NCH + PARTS - 1) / PARTS, HK = (KCH + PARTS - 1) / PARTS;
     constexpr bool SKIP = sizeof(T) == 4;  // matrix instructions bound float: none for what lies past K or N
     constexpr int VK = KCH * 4, VN = NCH * 4;          // vectors of a row
-    constexpr int PAD = sizeof(T) == 4 ? 1 : 2;  // spreads rows over the banks, for whole as for transposed reads
-    constexpr int PK = VK + PAD, PN = VN + PAD;
+    constexpr int PK = VK + S::PAD, PN = VN + S::PAD;  // pitches that spread rows over the banks, read either way
     // Vectors are dealt to threads by powers of two a row; a row of 6 or 7
     // chunks leaves some without.
     constexpr int DN = NCH > 4 ? 32 : VN;
-    constexpr int RB = fused_strips<T, KCH, NCH>(), ROWS = 64 * RB;
-    constexpr int LK = (ROWS * VK + 511) / 512, LN = (ROWS * DN + 511) / 512;
+    constexpr int RB = S::RB, ROWS = S::ROWS;
+    constexpr int LK = (ROWS * VK + THREADS - 1) / THREADS, LN = (ROWS * DN + THREADS - 1) / THREADS;
     __shared__ u32x4 w_lds[NCH * KC * PK];
     __shared__ u32x4 x_lds[ROWS * PK];
-    __shared__ u32x4 z_lds[ROWS * PN];
+    __shared__ u32x4 z_lds[PLANES][ROWS * PN];
     __shared__ f32x4 bias_lds[NCH * KC / 4];
 
     const int tid = threadIdx.x, wave = wave_id();
-    const int half = wave >> 2;
+    const int part = wave / S::STRIPS;
     const int wn = wave / WK, wk = wave % WK;
     const int64_t begin = blockIdx.x * a.rows_per_block;
     const int64_t end = begin + a.rows_per_block < a.rows ? begin + a.rows_per_block : a.rows;
@@ -91,11 +93,11 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
     const T* dy = static_cast<const T*>(a.dy);
     T* dx = static_cast<T*>(a.dx);
 
-    for (int i = tid; i < NCH * KC * VK; i += 512) {
+    for (int i = tid; i < NCH * KC * VK; i += THREADS) {
         const int n = i / VK, u = i % VK;
         w_lds[n * PK + u] = n < a.N ? load_row(w + (int64_t)n * a.K, u * E, a.K) : u32x4{0u, 0u, 0u, 0u};
     }
-    for (int n = tid; n < NCH * KC; n += 512)
+    for (int n = tid; n < NCH * KC; n += THREADS)
         reinterpret_cast<float*>(bias_lds)[n] =
             a.bias && n < a.N ? to_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
 
@@ -116,13 +118,13 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
     auto load = [&](int64_t m0) {  // rows past the end: the last row again
 #pragma unroll
         for (int i = 0; i < LK; ++i) {
-            const int u = i * 512 + tid;
+            const int u = i * THREADS + tid;
             const int64_t m = m0 + u / VK < end ? m0 + u / VK : end - 1;
             xr[i].issue(a.x, m, u % VK * E);
         }
 #pragma unroll
         for (int i = 0; i < LN; ++i) {
-            const int u = i * 512 + tid;
+            const int u = i * THREADS + tid;
             const int64_t m = m0 + u / DN < end ? m0 + u / DN : end - 1;
             yr[i] = issue_row<T, WIDE>(dy + m * a.ldy, u % DN * E, a.N);
         }
@@ -133,18 +135,18 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
         const bool whole = m0 + ROWS <= end;
 #pragma unroll
         for (int i = 0; i < LK; ++i) {
-            const int u = i * 512 + tid;
-            if (ROWS * VK % 512 != 0 && u >= ROWS * VK) break;
+            const int u = i * THREADS + tid;
+            if (ROWS * VK % THREADS != 0 && u >= ROWS * VK) break;
             u32x4 v = xr[i].finish_in(a.x, VK * E <= a.K, u % VK * E);
             x_lds[u / VK * PK + u % VK] = whole || m0 + u / VK < end ? v : zero;
         }
 #pragma unroll
         for (int i = 0; i < LN; ++i) {
-            const int u = i * 512 + tid;
-            if (ROWS * DN % 512 != 0 && u >= ROWS * DN) break;
+            const int u = i * THREADS + tid;
+            if (ROWS * DN % THREADS != 0 && u >= ROWS * DN) break;
             u32x4 v = yr[i];
             if (VN * E > a.N) v = finish_row<T, WIDE>(v, u % DN * E, a.N);
-            if (DN == VN || u % DN < VN) z_lds[u / DN * PN + u % DN] = whole || m0 + u / DN < end ? v : zero;
+            if (DN == VN || u % DN < VN) z_lds[0][u / DN * PN + u % DN] = whole || m0 + u / DN < end ? v : zero;
         }
     };
 
@@ -158,17 +160,17 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
         int lane = tid & 63;
         asm volatile("" : "+v"(lane));
         const int r = lane & 15, q = lane >> 4;
-        if (a.act != GS3D_ACT_NONE) {
+        if constexpr (ACT) {
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
-                const int strip = (b * 4 + (wave & 3)) * 16;
+                const int strip = (b * S::STRIPS + wave % S::STRIPS) * 16;
                 u32x4 xf[KCH];
 #pragma unroll
                 for (int c = 0; c < KCH; ++c) xf[c] = x_lds[(strip + r) * PK + c * 4 + q];
 #pragma unroll
                 for (int gi = 0; gi < HN; ++gi) {
-                    const int g = NCH == 1 ? 0 : 2 * gi + half;
-                    if (NCH == 1 && half != (RB == 2 ? b : 0)) break;  // one chunk: a strip each
+                    const int g = NCH == 1 ? 0 : PARTS * gi + part;
+                    if (NCH == 1 && part != (RB == 2 ? b : 0)) break;  // one chunk: a strip each
                     if (g >= NCH || (SKIP && g * KC >= a.N)) break;
                     f32x4 z[TG];
 #pragma unroll
@@ -180,13 +182,18 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
                             z[t] = multiply_chunk<T>(w_lds[tile_column<T>(g * TG + t, r) * PK + c * 4 + q], xf[c], z[t],
                                                      a.K - c * KC);
                     settle(z);
-                    u32x4& slot = z_lds[(strip + r) * PN + g * 4 + q];
+                    const int at = (strip + r) * PN + g * 4 + q;
                     float arg[E], grad[E];
-                    unpack<T>(slot, grad);
+                    unpack<T>(z_lds[0][at], grad);
 #pragma unroll
                     for (int i = 0; i < E; ++i) arg[i] = z[i / 4][i & 3];
                     pull_back(grad, arg, a.act);
-                    slot = pack<T>(grad);
+                    if constexpr (PLANES == 2) {
+                        z_lds[0][at] = take_high<T>(grad);
+                        z_lds[1][at] = pack<T>(grad);
+                    } else {
+                        z_lds[0][at] = pack<T>(grad);
+                    }
                 }
             }
             __syncthreads();
@@ -194,18 +201,12 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
         if (dx) {
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
-                const int strip = (b * 4 + (wave & 3)) * 16;
+                const int strip = (b * S::STRIPS + wave % S::STRIPS) * 16;
                 const int64_t m = m0 + strip + r;
-                // Float's twice as many vectors are read where they are used.
-                u32x4 dz[SKIP ? 1 : NCH];
-                if constexpr (!SKIP) {
-#pragma unroll
-                    for (int g = 0; g < NCH; ++g) dz[g] = z_lds[(strip + r) * PN + g * 4 + q];
-                }
 #pragma unroll
                 for (int ci = 0; ci < HK; ++ci) {
-                    const int c = KCH == 1 ? 0 : 2 * ci + half;
-                    if (KCH == 1 && half != (RB == 2 ? b : 0)) break;
+                    const int c = KCH == 1 ? 0 : PARTS * ci + part;
+                    if (KCH == 1 && part != (RB == 2 ? b : 0)) break;
                     if (c >= KCH || (SKIP && c * KC >= a.K)) break;
                     f32x4 out[TG];
 #pragma unroll
@@ -213,11 +214,11 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
 #pragma unroll
                     for (int g = 0; g < NCH; ++g) {
                         if (SKIP && g * KC >= a.N) break;
-                        if constexpr (SKIP) dz[0] = z_lds[(strip + r) * PN + g * 4 + q];
+                        const u32x4 dz = z_lds[0][(strip + r) * PN + g * 4 + q];
 #pragma unroll
                         for (int t = 0; t < TG; ++t)
                             out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, c * TG + t, lane),
-                                                       dz[SKIP ? 0 : g], out[t], a.N - g * KC);
+                                                       dz, out[t], a.N - g * KC);
                     }
                     settle(out);
                     float v[E];
@@ -232,11 +233,13 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
             for (int c = 0; c < ROWS / KC; ++c) {
                 // Where the tiles do not share out evenly the last one is taken
                 // again, and not stored.
-                u32x4 fz[TN], fx[TK];
+                u32x4 fz[PLANES][TN], fx[TK];
 #pragma unroll
                 for (int i = 0; i < TN; ++i) {
                     const int t = i * WN + wn;
-                    fz[i] = read_transposed<T, false>(z_lds, PN, c * KC, t < NT ? t : NT - 1, lane);
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p)
+                        fz[p][i] = read_transposed<T, false>(z_lds[p], PN, c * KC, t < NT ? t : NT - 1, lane);
                 }
 #pragma unroll
                 for (int j = 0; j < TK; ++j) {
@@ -244,11 +247,13 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
                     fx[j] = read_transposed<T, false>(x_lds, PK, c * KC, t < KT ? t : KT - 1, lane);
                 }
 #pragma unroll
-                for (int i = 0; i < TN; ++i) {
+                for (int p = 0; p < PLANES; ++p)
 #pragma unroll
-                    for (int j = 0; j < TK; ++j) acc[i][j] = multiply<T>(fz[i], fx[j], acc[i][j]);
-                    acc_b[i] = multiply<T>(fz[i], ones, acc_b[i]);
-                }
+                    for (int i = 0; i < TN; ++i) {
+#pragma unroll
+                        for (int j = 0; j < TK; ++j) acc[i][j] = multiply<T>(fz[p][i], fx[j], acc[i][j]);
+                        acc_b[i] = multiply<T>(fz[p][i], ones, acc_b[i]);
+                    }
             }
         }
         __syncthreads();  // the tiles' readers are done
@@ -259,7 +264,7 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
 #pragma unroll
     for (int i = 0; i < TN; ++i) settle(acc[i]);
     settle(acc_b);
-    float* part = a.part + (int64_t)blockIdx.x * ((int64_t)a.N * a.K + a.N);
+    float* out = a.part + (int64_t)blockIdx.x * ((int64_t)a.N * a.K + a.N);
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
@@ -269,9 +274,9 @@ __global__ __launch_bounds__(512, (fused_waves<T, KCH, NCH>())) void linear_bwd_
 #pragma unroll
             for (int j = 0; j < TK; ++j) {
                 const int k = (j * WK + wk) * 16 + r;
-                if (k < a.K) part[(int64_t)n * a.K + k] = acc[i][j][e];
+                if (k < a.K) out[(int64_t)n * a.K + k] = acc[i][j][e];
             }
-            if (wk == 0 && r == 0) part[(int64_t)a.N * a.K + n] = acc_b[i][e];
+            if (wk == 0 && r == 0) out[(int64_t)a.N * a.K + n] = acc_b[i][e];
         }
 }
 
@@ -298,18 +303,32 @@ static bool fused_fits(int K, int N) {
     return sizeof(T) == 4 || fused_chunks_k<T>(K) * fused_chunks_n<T>(N) <= 16;
 }
 
+template <class T, bool Q8, int KCH, int NCH, bool WIDE, bool ACT>
+static void launch_fused_act(LinearFused a, int blocks, hipStream_t stream) {
+    using S = FusedShape<T, KCH, NCH, ACT>;
+    // Half as many blocks where one fills a compute unit (the scratch was
+    // sized for two).
+    if (!S::TWO && blocks > 256) {
+        a.rows_per_block = (a.rows_per_block * blocks / 256 + 63) / 64 * 64;
+        blocks = (int)((a.rows + a.rows_per_block - 1) / a.rows_per_block);
+    }
+    *a.blocks = blocks;
+    hipLaunchKernelGGL((linear_bwd_fused_kernel<T, Q8, KCH, NCH, WIDE, ACT>), dim3((unsigned)blocks),
+                       dim3(S::WAVES * 64), 0, stream, a);
+}
 template <class T, bool Q8, int KCH, int NCH>
 static void launch_fused_as(const LinearFused& a, int blocks, hipStream_t stream) {
     constexpr int LEAST = sizeof(T) == 4 ? 2 : 1;
+    const bool act = a.act != GS3D_ACT_NONE;
     if constexpr (KCH == LEAST || NCH == LEAST) {
         if (a.K < VEC<T> || a.N < VEC<T>) {  // rows shorter than a vector
-            hipLaunchKernelGGL((linear_bwd_fused_kernel<T, Q8, KCH, NCH, false>), dim3((unsigned)blocks), dim3(512), 0,
-                               stream, a);
+            if (act) launch_fused_act<T, Q8, KCH, NCH, false, true>(a, blocks, stream);
+            else launch_fused_act<T, Q8, KCH, NCH, false, false>(a, blocks, stream);
             return;
         }
     }
-    hipLaunchKernelGGL((linear_bwd_fused_kernel<T, Q8, KCH, NCH, true>), dim3((unsigned)blocks), dim3(512), 0, stream,
-                       a);
+    if (act) launch_fused_act<T, Q8, KCH, NCH, true, true>(a, blocks, stream);
+    else launch_fused_act<T, Q8, KCH, NCH, true, false>(a, blocks, stream);
 }
 template <class T, bool Q8, int KCH>
 static void launch_fused_n(const LinearFused& a, int blocks, hipStream_t stream) {
