@@ -325,10 +325,10 @@ GS3D_DEV void q8_store(int8_t* row, int at, int count, const uint32_t (&words)[N
     }
 }
 
-// One lane's vector of a row written in 8 bits, from channel `at` on; 32 /
-// VEC<T> neighbouring lanes, all active, hold a block (zeros past the row's
-// end).  `live`: the row is there.
-template <class T>
+// One lane's vector of a row written in 8 bits, from channel `at` on; LANES
+// neighbouring lanes, all active, hold a block (32 / VEC<T> with zeros past the
+// row's end, or fewer that cover all of a row).  `live`: the row is there.
+template <class T, int LANES = 32 / VEC<T>>
 GS3D_DEV void q8_keep(const float (&v)[VEC<T>], int8_t* codes, uint8_t* scales, int64_t row, int at, int channels,
                       bool live) {
     constexpr int E = VEC<T>;
@@ -338,7 +338,7 @@ GS3D_DEV void q8_keep(const float (&v)[VEC<T>], int8_t* codes, uint8_t* scales, 
         const uint32_t m = magnitude_bits(v[i]);
         largest = m > largest ? m : largest;
     }
-    const uint32_t byte = q8_scale_byte<T>(q8_block_max<32 / E>(largest));
+    const uint32_t byte = q8_scale_byte<T>(q8_block_max<LANES>(largest));
     uint32_t words[E / 4];
 #pragma unroll
     for (int i = 0; i < E / 4; ++i) words[i] = q8_word(v + 4 * i, byte);

@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT, WIDE>())) v
                     const int64_t m = m0 + i * (64 / VK) + lane / VK;
                     float f[E];
                     unpack<T>(v, f);
-                    q8_keep<T>(f, a.keep_codes, a.keep_scales, m, lane % VK * E, a.K, whole.value || m < end);
+                    q8_keep<T, (VK < 32 / E ? VK : 32 / E)>(f, a.keep_codes, a.keep_scales, m, lane % VK * E, a.K, whole.value || m < end);
                 }
             }
         }
