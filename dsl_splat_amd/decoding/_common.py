@@ -2,6 +2,7 @@
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from ..runtime import abi, native
 
@@ -60,6 +61,15 @@ def rows_of(x: Tensor) -> tuple[Tensor, int]:
 
 def scratch(nbytes: int, device: torch.device) -> Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+
+
+def recorded(*tensors: Tensor | None) -> bool:
+    """Whether autograd has to see a call on these tensors.  One that it need
+    not see runs without a node (10 us rather than 15 of host time); within
+    forward-mode differentiation all are shown, and refused by the node."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def launch(name: str, args, device: torch.device, *rest) -> None:

@@ -11,8 +11,9 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from ..runtime import abi, native
-from ._common import (DTYPES, activation_code, check_checkpoint, check_input, check_like, launch, rows_of, scratch)
-from .activations import empty_quantized
+from ._common import (DTYPES, activation_code, check_checkpoint, check_input, check_like, launch, recorded, rows_of,
+                      scratch)
+from .activations import QuantizedActivations, empty_quantized
 
 
 def _scratch(shape, groups: int, dtype: int, device: torch.device) -> Tensor:
@@ -20,33 +21,41 @@ def _scratch(shape, groups: int, dtype: int, device: torch.device) -> Tensor:
     return scratch(native.query("gs3d_group_norm_scratch_bytes", images, pixels, shape[-1], groups, dtype), device)
 
 
+def _forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, groups: int, eps: float, activation: int,
+             quantized: QuantizedActivations | None) -> tuple[Tensor, Tensor, int, Tensor | None, Tensor | None, Tensor]:
+    """(result, x as rows, their stride, weight, bias, statistics), the inputs
+    as the kernels read them; where `quantized` is given x's 8-bit form goes
+    there."""
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    images, channels = math.prod(x.shape[:-3]), x.shape[-1]
+    rows, x_stride = rows_of(x)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    statistics = torch.empty((images, groups, 2), dtype=torch.float32, device=x.device)
+    a = abi.GroupNormArgs()
+    a.images, a.pixels, a.channels, a.groups = images, x.shape[-3] * x.shape[-2], channels, groups
+    a.dtype, a.activation, a.eps = DTYPES[x.dtype], activation, eps
+    a.x, a.x_stride = native.ptr(rows), x_stride
+    a.weight, a.bias, a.y, a.statistics = (native.ptr(t) for t in (weight, bias, y, statistics))
+    if quantized is not None:
+        a.codes, a.scales = native.ptr(quantized.codes), native.ptr(quantized.scales)
+    if x.numel():
+        work = _scratch(x.shape, groups, a.dtype, x.device)
+        launch("gs3d_group_norm_fwd", ctypes.byref(a), x.device, native.ptr(work), work.numel())
+    return y, rows, x_stride, weight, bias, statistics
+
+
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor | None, bias: Tensor | None, groups: int, eps: float,
-                activation: int, checkpoint: str | None, grad_enabled: bool) -> Tensor:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        images, channels = math.prod(x.shape[:-3]), x.shape[-1]
-        rows, x_stride = rows_of(x)
-        weight = None if weight is None else weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        statistics = torch.empty((images, groups, 2), dtype=torch.float32, device=x.device)
-        a = abi.GroupNormArgs()
-        a.images, a.pixels, a.channels, a.groups = images, x.shape[-3] * x.shape[-2], channels, groups
-        a.dtype, a.activation, a.eps = DTYPES[x.dtype], activation, eps
-        a.x, a.x_stride = native.ptr(rows), x_stride
-        a.weight, a.bias, a.y, a.statistics = (native.ptr(t) for t in (weight, bias, y, statistics))
-        save = grad_enabled and any(ctx.needs_input_grad[:3])
+                activation: int, checkpoint: str | None) -> Tensor:
+        quantized = empty_quantized(x) if checkpoint is not None else None
+        y, rows, x_stride, weight, bias, statistics = _forward(x, weight, bias, groups, eps, activation, quantized)
         kept: tuple[Tensor | None, ...] = (rows, None, None)
-        if save and checkpoint is not None:
-            quantized = empty_quantized(x)
+        if quantized is not None:
             kept = (None, quantized.codes, quantized.scales)
-            a.codes, a.scales = native.ptr(quantized.codes), native.ptr(quantized.scales)
-        if x.numel():
-            work = _scratch(x.shape, groups, a.dtype, x.device)
-            launch("gs3d_group_norm_fwd", ctypes.byref(a), x.device, native.ptr(work), work.numel())
-        if save:
-            ctx.save_for_backward(*kept, weight, bias, statistics)
-            ctx.shape, ctx.x_stride, ctx.groups, ctx.activation = x.shape, x_stride, groups, activation
+        ctx.save_for_backward(*kept, weight, bias, statistics)
+        ctx.shape, ctx.x_stride, ctx.groups, ctx.activation = x.shape, x_stride, groups, activation
         ctx.set_materialize_grads(False)
         return y
 
@@ -54,7 +63,7 @@ class _GroupNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx: Any, gradient: Tensor | None) -> tuple[Tensor | None, ...]:
         if gradient is None:
-            return (None,) * 8
+            return (None,) * 7
         x, codes, scales, weight, bias, statistics = ctx.saved_tensors
         channels = ctx.shape[-1]
         upstream, stride = rows_of(gradient)
@@ -76,7 +85,7 @@ class _GroupNorm(torch.autograd.Function):
             for g in grads:
                 if g is not None:
                     g.zero_()
-        return (*grads, None, None, None, None, None)
+        return (*grads, None, None, None, None)
 
 
 def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tensor | None = None, *,
@@ -105,4 +114,6 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
         raise ValueError(f"eps must be positive and finite, got {eps!r}")
     code = activation_code(activation)
     check_checkpoint(checkpoint)
-    return _GroupNorm.apply(x, weight, bias, int(groups), float(eps), code, checkpoint, torch.is_grad_enabled())
+    if not recorded(x, weight, bias):
+        return _forward(x, weight, bias, int(groups), float(eps), code, None)[0]
+    return _GroupNorm.apply(x, weight, bias, int(groups), float(eps), code, checkpoint)
