@@ -18,6 +18,12 @@
 //
 // Moments are merged as (count, mean, M2) throughout: an image whose mean is
 // far from zero loses no digits to a difference of squares.
+//
+// HBM bounds all of it: 4 x 1920 x 1080 x 64 floats, statistics 384 us (5.5
+// TB/s), apply 827 and sums 736 (5.1, 5.8), gradient 1232 (5.2).  The second
+// passes walk backwards over each strip, whose end the first one left in the
+// cache (1 to 2%).  One pass would need an image to stay on the chip: a launch
+// per image, so that the last-level cache held it, cost more than it saved.
 #include "decode.hpp"
 
 namespace gs3d {

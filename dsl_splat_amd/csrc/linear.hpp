@@ -5,7 +5,9 @@
 //   linear_stream_kernel     rows times weights that lie in LDS whole, while the
 //                            rows stream past: every product whose contracted
 //                            dimension has at most 4 chunks
-//   linear_rows_kernel       the same for longer ones, the weights in steps
+//   linear_tile_kernel       longer ones of 16-bit types: 64 whole rows in LDS
+//                            against weights that pack_weights_kernel laid out
+//   linear_rows_kernel       the other longer ones: rows and weights in steps
 //   linear_bwd_fused_kernel  the whole backward pass in one (linear_fused.hpp),
 //                            where its weights and their gradient fit a block
 //   linear_gradw_kernel      otherwise: dW = dz^T x and db = sum dz, split over
@@ -16,8 +18,7 @@
 // those of the backward (EPI 1) in dz = dy act'(x W^T + b), z computed again
 // rather than kept.
 // Products of 16-bit types go through matrix instructions with sums in 32
-// bits.  dz is rounded to the element type once, as the operand of the two
-// products that follow it.
+// bits.  dz enters the products after it as decode.hpp says at SPLIT.
 #pragma once
 
 #include "linear_fused.hpp"
@@ -105,7 +106,7 @@ template <class T, bool Q8, int EPI, int KCH, int NT, bool WIDE>
 constexpr int stream_waves() {
     const int wide = sizeof(T) == 4 ? 2 : 1;  // float holds twice the vectors
     const int vectors =
-        wide * (2 * KCH + (EPI != 0 ? NT / 2 : 0)) + (KEEPS_LOW<T, EPI> ? NT / 2 + 1 : 0) + (WIDE ? 0 : 3);
+        wide * (2 * KCH + (EPI != 0 ? NT / 2 : 0)) + (KEEPS_LOW<T, EPI> ? NT / 2 + 1 : 0) + (WIDE ? 0 : 5);
     return vectors <= 4 ? 6 : vectors <= 8 ? 5 : vectors <= 12 ? 4 : vectors <= 16 ? 3 : 2;
 }
 
@@ -191,7 +192,8 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT, WIDE>())) v
                     const int64_t m = m0 + i * (64 / VK) + lane / VK;
                     float f[E];
                     unpack<T>(v, f);
-                    q8_keep<T, (VK < 32 / E ? VK : 32 / E)>(f, a.keep_codes, a.keep_scales, m, lane % VK * E, a.K, whole.value || m < end);
+                    q8_keep<T, (VK < 32 / E ? VK : 32 / E)>(f, a.keep_codes, a.keep_scales, m, lane % VK * E, a.K,
+                                                            whole.value || m < end);
                 }
             }
         }
@@ -264,13 +266,14 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT, WIDE>())) v
     if (m0 < end) strip(m0, Flag<false>{});
 }
 
-// Longer contracted dimensions, where the products count more than the bytes:
-// a block of 4 wavefronts computes 64 RS rows x 16 NT columns.  CH chunks of
+// Longer contracted dimensions, where the products count more than the bytes,
+// of float, of a few rows, beyond 512 channels or into a few columns: a block of 4 wavefronts computes 64 RS rows x 16 NT columns.  CH chunks of
 // the weights at a time go through LDS, twice buffered, so a step has one
 // barrier; a fragment read from there serves the RS strips of a wavefront
 // (the LDS port, 128 bytes a clock, would bound RS = 1: 8 clocks a fragment
 // and wavefront, 16 clocks a matrix instruction).  The next step's operands
-// are loaded while this one's are multiplied.
+// are loaded while this one's are multiplied.  1.44 M rows of float, 128 to 64
+// channels: 360 us, 66 TFLOP/s of the 152 that a large product reaches, 3.1 TB/s.
 template <class T, bool Q8, int EPI, int RS, int NT, bool WIDE>
 __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     constexpr int E = VEC<T>;
@@ -442,9 +445,12 @@ static int64_t packed_vectors(int N, int K) {
 // 64 whole rows of x into LDS and goes over all N columns: a wavefront takes 64
 // of them at a time against the 64 rows (4 x 4 tiles), its fragments of W,
 // packed, from the L2, where they stay.  After the rows have come the
-// wavefronts never wait for one another.  TILE_NOTE
+// wavefronts never wait for one another.  268177 rows, 256 to 512 channels of
+// bfloat16: 145 us, 485 TFLOP/s and 2.8 TB/s, a third and a half of what either
+// reaches alone: a block's loads, products and activations follow one another,
+// and only the 2 or 3 blocks that its LDS leaves room for overlap them.
 template <class T, bool Q8, int EPI, int KCH>
-__global__ __launch_bounds__(256, KCH * (int)sizeof(T) > 64 ? 1 : KCH * (int)sizeof(T) > 16 || EPI != 0 ? 2 : 3)
+__global__ __launch_bounds__(256, KCH > 8 || EPI != 0 ? 2 : 3)
 void linear_tile_kernel(LinearRows a) {
     constexpr int E = VEC<T>;
     constexpr int KC = CHUNK<T>;
@@ -796,25 +802,33 @@ static void launch_long_as(LinearRows a, hipStream_t stream) {
 }
 
 // Few rows: narrow column tiles, so that many compute units read the weights
-// at once.
+// at once (one row, 32 to 512 channels of float: 2.9 us, in wide tiles 6.1; 1000
+// rows, 512 to 512 of bfloat16: 7.0 and 12.6).
 static bool few_rows(const LinearRows& a) { return a.rows <= 1024; }
 
+// The tile's width: 128 columns read a row once, 64 leave a float tile's LDS
+// room for twice the wavefronts (1.44 M rows of float, 32 to 128 channels: 224
+// us at 64 columns, 260 at 128; 33 to 97: 242 and 308; 32 to 97: 268 and 256).
 template <class T, bool Q8, int EPI, int KCH>
 static void launch_stream(const LinearRows& a, hipStream_t stream) {
-    constexpr int E = VEC<T>;
+    constexpr int E = VEC<T>, MOST = sizeof(T) == 4 ? 4 : 8;
     if (a.K < E || a.N < E) {  // rows shorter than a vector, in or out
         if (a.N <= 32 || few_rows(a)) return launch_stream_as<T, Q8, EPI, KCH, 2, false>(a, stream);
-        if constexpr (KCH == 1) return launch_stream_as<T, Q8, EPI, 1, 8, false>(a, stream);
+        if constexpr (KCH == 1) return launch_stream_as<T, Q8, EPI, 1, MOST, false>(a, stream);
     }
     if (a.N <= 32 || few_rows(a)) launch_stream_as<T, Q8, EPI, KCH, 2, true>(a, stream);
     else if (a.N <= 64) launch_stream_as<T, Q8, EPI, KCH, 4, true>(a, stream);
-    else launch_stream_as<T, Q8, EPI, KCH, 8, true>(a, stream);
+    else launch_stream_as<T, Q8, EPI, KCH, MOST, true>(a, stream);
 }
-// Products that the tile kernel takes: more than 4 chunks of K, as many as a
-// block's rows find room for, and enough rows to fill the blocks.
+// Products that the tile kernel takes: of 16-bit types, more than 4 chunks of K,
+// as many as a block's rows find room for, and enough rows to fill the blocks.
+// It and the rows kernel in its place (us, packing included): 268177 rows, 256
+// to 512 channels of bfloat16, the forward's and the backward's two products
+// 594 and 662; 1100 rows, 512 to 64: 12.8 and 14.3; 2000 rows, 256 to 256: 10.5
+// and 8.7.  Float's rows take twice the LDS: 1.44 M rows, 128 to 64: 529 and 365.
 template <class T>
 static bool tiled(int64_t rows, int K, int N) {
-    return K > 4 * CHUNK<T> && K <= 512 && rows > 1024 && N >= VEC<T>;
+    return sizeof(T) == 2 && K > 4 * CHUNK<T> && K <= 512 && rows > 1024 && N >= VEC<T>;
 }
 template <class T, bool Q8, int EPI, int KCH>
 static void launch_tile(const LinearRows& a, hipStream_t stream) {
@@ -832,16 +846,16 @@ static void launch_long(const LinearRows& a, hipStream_t stream) {
 // product; TRANSPOSED: a.w is K x N.
 template <class T, bool Q8, int EPI, bool TRANSPOSED>
 static void launch_rows(LinearRows a, void* packed, hipStream_t stream) {
-    if (tiled<T>(a.rows, a.K, a.N)) {
-        const int64_t vectors = packed_vectors<T>(a.N, a.K);
-        hipLaunchKernelGGL((pack_weights_kernel<T, TRANSPOSED>), dim3((unsigned)(vectors / 256)), dim3(256), 0, stream,
-                           static_cast<const T*>(a.w), a.N, a.K, (a.K + CHUNK<T> - 1) / CHUNK<T>,
-                           static_cast<u32x4*>(packed));
-        a.w = packed;
-        const int chunks = (a.K + CHUNK<T> - 1) / CHUNK<T>;
-        if (chunks <= 8) return launch_tile<T, Q8, EPI, 8>(a, stream);
-        if (chunks <= 16) return launch_tile<T, Q8, EPI, 16>(a, stream);
-        if constexpr (sizeof(T) == 4) return launch_tile<T, Q8, EPI, 32>(a, stream);
+    if constexpr (sizeof(T) == 2) {
+        if (tiled<T>(a.rows, a.K, a.N)) {
+            const int64_t vectors = packed_vectors<T>(a.N, a.K);
+            const int chunks = (a.K + CHUNK<T> - 1) / CHUNK<T>;
+            hipLaunchKernelGGL((pack_weights_kernel<T, TRANSPOSED>), dim3((unsigned)(vectors / 256)), dim3(256), 0,
+                               stream, static_cast<const T*>(a.w), a.N, a.K, chunks, static_cast<u32x4*>(packed));
+            a.w = packed;
+            if (chunks <= 8) return launch_tile<T, Q8, EPI, 8>(a, stream);
+            return launch_tile<T, Q8, EPI, 16>(a, stream);
+        }
     }
     if constexpr (TRANSPOSED) {
         T* wt = static_cast<T*>(packed);
