@@ -67,7 +67,7 @@ def test_entry_points_check_their_arguments(make, name, scratch, changes):
     if scratch:
         a = make()
         if name == "gs3d_linear_fwd":
-            a.rows, a.inner, a.x_stride, a.dtype = 100_000, 300, 300, abi.DTYPE_BF16  # packed weights
+            a.rows, a.inner, a.outer, a.x_stride, a.dtype = 100_000, 300, 16, 300, abi.DTYPE_BF16  # packed weights
         assert call(ctypes.byref(a), P, 1, None) == abi.GS3D_ERR_SCRATCH
         assert call(ctypes.byref(a), None, 1 << 40, None) == abi.GS3D_ERR_SCRATCH
 
