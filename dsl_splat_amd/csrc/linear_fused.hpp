@@ -21,18 +21,22 @@ struct LinearFused {
 };
 
 // How a backward kernel of KCH x NCH chunks lies on a compute unit: two blocks
-// of 8 wavefronts where their LDS fits, of 128 rows or 64; else one of 16, the
-// weights once for all of them.  Four wavefronts a SIMD either way.
+// of 8 wavefronts where their LDS fits, of 128, 64 or 32 rows at a time, whose
+// barriers leave each other's work alone; else one of 16, the weights once for
+// all of them.  Four wavefronts a SIMD either way.  Two blocks of 32 rows and
+// one of 128 (us, silu): 1.92 M rows of bfloat16, 128 to 128 channels, 599 and
+// 639; 1 M rows, 64 to 256: 355 and 407; float, 64 to 128: 692 and 773.
 template <class T, int KCH, int NCH, bool ACT>
 struct FusedShape {
     static constexpr int PLANES = SPLIT<T> && ACT ? 2 : 1;
     static constexpr int PAD = sizeof(T) == 4 ? 1 : 2;
     static constexpr int FIXED = NCH * CHUNK<T> * ((KCH * 4 + PAD) * 16 + 4);
     static constexpr int ROW = (KCH * 4 + PAD + PLANES * (NCH * 4 + PAD)) * 16;
-    static constexpr bool TWO = FIXED + 64 * ROW <= 81920;
+    static constexpr bool TWO = FIXED + 32 * ROW <= 81920;
     static constexpr int WAVES = TWO ? 8 : 16;
-    static constexpr int ROWS = FIXED + 128 * ROW <= (TWO ? 81920 : 163840) ? 128 : 64;
-    static constexpr int STRIPS = ROWS == 128 && WAVES == 16 ? 8 : 4;  // of 16 rows, taken at a time
+    static constexpr int ROOM = TWO ? 81920 : 163840;
+    static constexpr int ROWS = FIXED + 128 * ROW <= ROOM ? 128 : FIXED + 64 * ROW <= ROOM ? 64 : 32;
+    static constexpr int STRIPS = ROWS == 128 && WAVES == 16 ? 8 : ROWS == 32 ? 2 : 4;  // of 16 rows, taken at a time
     static constexpr int PARTS = WAVES / STRIPS;                       // wavefronts that share a strip
     static constexpr int RB = ROWS / (16 * STRIPS);
 };
@@ -59,10 +63,10 @@ struct FusedShape {
 // Bytes bound it where K and N are small (x and dy in, dx out), the vector
 // units where the slope is dear; four wavefronts a SIMD let one's loads and
 // slopes run under another's products.  1.92 M rows of bfloat16, 32 to 128
-// channels: 187 us without an activation (2.0 TB/s), 316 with gelu; 128 to 128
-// with silu from 8 bits 502; 1.44 M rows of float, 33 to 97: 656, 70 TFLOP/s of
+// channels: 187 us without an activation (3.9 TB/s), 316 with gelu; 128 to 128
+// with silu from 8 bits 498; 1.44 M rows of float, 33 to 97: 656, 70 TFLOP/s of
 // 152.  As separate products instead (us, forward and backward): 128 to 128
-// 1151, here 854; float 33 to 97 1528, here 1029; 1000 rows, 64 to 64 of
+// 1151, here 825; float 33 to 97 1528, here 1029; 1000 rows, 64 to 64 of
 // float16 24.8, here 15.2.
 template <class T, bool Q8, int KCH, int NCH, bool WIDE, bool ACT>
 __global__ __launch_bounds__((FusedShape<T, KCH, NCH, ACT>::WAVES * 64), 4)
