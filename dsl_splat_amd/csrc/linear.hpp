@@ -613,7 +613,7 @@ struct LinearGradW {
     const void* low;  // what dz leaves, rows x N, or NULL
     int64_t ldz;
     int64_t rows, rows_per_split;
-    int N, n_tiles, k_tiles;
+    int N, n_tiles, k_tiles, splits;
     float* part;     // splits x (N K + N)
     int K;
 };
@@ -634,11 +634,11 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
     __shared__ u32x4 z_lds[PLANES][MR * PZ];
     __shared__ u32x4 x_lds[MR * PX];
 
-    int64_t b = blockIdx.x;
-    const int kt = (int)(b % a.k_tiles);
-    b /= a.k_tiles;
-    const int nt = (int)(b % a.n_tiles);
-    const int split = (int)(b / a.n_tiles);
+    // A split's tiles run on one XCD, whose L2 then holds its rows once.
+    const int local = blockIdx.x >> 3, tiles = a.n_tiles * a.k_tiles;
+    const int split = local / tiles * 8 + (blockIdx.x & 7);
+    if (split >= a.splits) return;
+    const int kt = local % tiles % a.k_tiles, nt = local % tiles / a.k_tiles;
     const int n0 = nt * 32 * A, k0 = kt * 32 * B;
     const int64_t begin = split * a.rows_per_split;
     const int64_t end = begin + a.rows_per_split < a.rows ? begin + a.rows_per_split : a.rows;
@@ -873,7 +873,7 @@ static void launch_rows(LinearRows a, void* packed, hipStream_t stream) {
 
 template <class T, bool Q8, int A, int B>
 static void launch_gradw_as(const LinearGradW& a, int splits, hipStream_t stream) {
-    const dim3 grid((unsigned)(a.n_tiles * a.k_tiles * splits));
+    const dim3 grid((unsigned)(a.n_tiles * a.k_tiles * ((splits + 7) / 8 * 8)));
     if constexpr (SPLIT<T>) {
         if (a.low) {
             hipLaunchKernelGGL((linear_gradw_kernel<T, Q8, A, B, 2>), grid, dim3(256), 0, stream, a);
@@ -1002,7 +1002,7 @@ static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t 
             launch_rows<T, false, 0, true>(a, scratch + at.wt, stream);
         }
         if (params) {
-            LinearGradW a{x, dz, low, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, part, g.inner};
+            LinearGradW a{x, dz, low, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, p.splits, part, g.inner};
             launch_gradw<T, Q8>(a, p.splits, stream);
         }
     }
