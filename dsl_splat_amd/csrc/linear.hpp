@@ -267,13 +267,14 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT, WIDE>())) v
 }
 
 // Longer contracted dimensions, where the products count more than the bytes,
-// of float, of a few rows, beyond 512 channels or into a few columns: a block of 4 wavefronts computes 64 RS rows x 16 NT columns.  CH chunks of
-// the weights at a time go through LDS, twice buffered, so a step has one
-// barrier; a fragment read from there serves the RS strips of a wavefront
-// (the LDS port, 128 bytes a clock, would bound RS = 1: 8 clocks a fragment
-// and wavefront, 16 clocks a matrix instruction).  The next step's operands
-// are loaded while this one's are multiplied.  1.44 M rows of float, 128 to 64
-// channels: 360 us, 66 TFLOP/s of the 152 that a large product reaches, 3.1 TB/s.
+// of float, of a few rows, beyond 512 channels or into a few columns: a block
+// of 4 wavefronts computes 64 RS rows x 16 NT columns.  CH chunks of the
+// weights at a time go through LDS, twice buffered, so a step has one barrier;
+// a fragment read from there serves the RS strips of a wavefront (the LDS port,
+// 128 bytes a clock, would bound RS = 1: 8 clocks a fragment and wavefront, 16
+// clocks a matrix instruction).  The next step's operands are loaded while this
+// one's are multiplied.  1.44 M rows of float, 128 to 64 channels: 360 us, 66
+// TFLOP/s of the 152 that a large product reaches, 3.1 TB/s.
 template <class T, bool Q8, int EPI, int RS, int NT, bool WIDE>
 __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     constexpr int E = VEC<T>;
@@ -349,7 +350,8 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
 #pragma unroll
         for (int s = 0; s < RS; ++s)
 #pragma unroll
-            for (int c = 0; c < CH; ++c) xc[s][c] = xr[s][c].finish_in(a.x, k0 + c * KC + KC <= a.K, k0 + c * KC + q * E);
+            for (int c = 0; c < CH; ++c)
+                xc[s][c] = xr[s][c].finish_in(a.x, k0 + c * KC + KC <= a.K, k0 + c * KC + q * E);
         __syncthreads();
         const bool more = k0 + CH * KC < a.K;
         if (more) load(k0 + CH * KC);
@@ -1002,7 +1004,8 @@ static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t 
             launch_rows<T, false, 0, true>(a, scratch + at.wt, stream);
         }
         if (params) {
-            LinearGradW a{x, dz, low, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, p.splits, part, g.inner};
+            LinearGradW a{x, dz, low, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, p.splits, part,
+                          g.inner};
             launch_gradw<T, Q8>(a, p.splits, stream);
         }
     }
