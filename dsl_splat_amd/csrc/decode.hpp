@@ -455,13 +455,10 @@ GS3D_DEV int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
 
 // ---------------------------------------------------------------------------
 // A gradient dz = dy act'(z) is computed in 32 bits and then an operand of two
-// matrix products.  Rounded once to 16 bits it makes the error of dx 1.33 to
-// 1.41 times, that of dW and db 1.34 to 1.53 times what rounding the results
-// alone gives (relu, silu and gelu, 100000 rows).  dW, which a training step
-// adds up over many calls, takes dz as two 16-bit values, high and low, and is
-// then as exact as its own rounding; dx takes the high one.  At 128 to 128
-// channels of bfloat16 and 1.92 M rows: one value 387 us, the low one in dW
-// 498 us, in dx as well 54 us more.  Float, and dy itself where there is no
+// matrix products.  Rounded once to 16 bits it makes the error of dx 1.41
+// times, that of dW and db 1.34 to 1.53 times what rounding the results alone
+// gives.  Both products take dz as two 16-bit values, high and low, and are
+// then as exact as their own rounding.  Float, and dy itself where there is no
 // activation, are one value.
 // ---------------------------------------------------------------------------
 template <class T>

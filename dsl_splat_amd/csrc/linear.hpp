@@ -18,7 +18,9 @@
 // those of the backward (EPI 1) in dz = dy act'(x W^T + b), z computed again
 // rather than kept.
 // Products of 16-bit types go through matrix instructions with sums in 32
-// bits.  dz enters the products after it as decode.hpp says at SPLIT.
+// bits.  dz enters the products after it as decode.hpp says at SPLIT: a row of
+// its N high halves and then its N low ones, so that dx = dz W is the product
+// of that row, twice as long, with W^T beside itself.
 #pragma once
 
 #include "linear_fused.hpp"
@@ -31,8 +33,8 @@ struct LinearRows {
     const void* bias;    // N or NULL
     const void* other;   // EPI 1: dy; EPI 2: residual
     int64_t ldo;
-    void* y;             // rows x N
-    void* low;           // EPI 1 of 16-bit types: what y leaves of dz, rows x N
+    void* y;             // rows x N; EPI 1 of 16-bit types: x 2 N, the second half what the first leaves of dz
+    int64_t ldy;
     int64_t rows;
     int K, N, act, n_tiles, strips;
     int8_t* keep_codes;  // where the rows of x are kept in 8 bits, or NULL
@@ -83,10 +85,12 @@ GS3D_DEV void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// A wavefront's strip of 16 rows x VP vectors, in LDS at pitch PO, to rows from
-// `first` on and columns from n0 on, whole row segments an instruction.
+// A wavefront's strip of 16 rows x VP vectors, in LDS at pitch PO, to rows of N
+// columns from `first` on and columns from n0 on, whole row segments an
+// instruction.
 template <class T, int VP, int PO, class Whole>
-GS3D_DEV void store_strip(const u32x4* strip, T* y, int64_t first, int64_t end, int n0, int N, int lane, Whole) {
+GS3D_DEV void store_strip(const u32x4* strip, T* y, int64_t ldy, int64_t first, int64_t end, int n0, int N, int lane,
+                          Whole) {
     constexpr int E = VEC<T>;
     wave_fence();
     const int vec = lane % VP, at = n0 + vec * E;
@@ -95,8 +99,8 @@ GS3D_DEV void store_strip(const u32x4* strip, T* y, int64_t first, int64_t end, 
         const int row = i * (64 / VP) + lane / VP;
         const u32x4 raw = strip[row * PO + vec];
         const int64_t to = first + row;
-        if (Whole::value && n0 + VP * E <= N) store16(y + to * N + at, raw);
-        else if (to < end) store_row(y + to * N, at, N, raw);
+        if (Whole::value && n0 + VP * E <= N) store16(y + to * ldy + at, raw);
+        else if (to < end) store_row(y + to * ldy, at, N, raw);
     }
     wave_fence();
 }
@@ -247,18 +251,18 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT, WIDE>())) v
             const int64_t m = m0 + r;
             if (staged) slot = raw;
             else if (whole.value || m < end) {
-                store_chunk(y + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
+                store_chunk(y + m * a.ldy, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
                 if constexpr (KEEPS_LOW<T, EPI>)
-                    store_chunk(static_cast<T*>(a.low) + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, low[g]);
+                    store_chunk(y + a.N + m * a.ldy, n0 + g * KC, n0 + g * KC + q * E, a.N, low[g]);
             }
         }
-        if (staged) store_strip<T, VP, PO>(mine, y, m0, end, n0, a.N, lane, whole);
+        if (staged) store_strip<T, VP, PO>(mine, y, a.ldy, m0, end, n0, a.N, lane, whole);
         else wave_fence();
         if constexpr (KEEPS_LOW<T, EPI>) {
             if (staged) {
 #pragma unroll
                 for (int g = 0; g < G; ++g) mine[r * PO + g * 4 + q] = low[g];
-                store_strip<T, VP, PO>(mine, static_cast<T*>(a.low), m0, end, n0, a.N, lane, whole);
+                store_strip<T, VP, PO>(mine, y + a.N, a.ldy, m0, end, n0, a.N, lane, whole);
             }
         }
     };
@@ -394,31 +398,32 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
             raw = linear_end<T, EPI, E>(a, z, raw, low[g]);
             if (staged) strip[r * PO + g * 4 + q] = raw;
             else if (m < a.rows) {
-                store_chunk(y + m * a.N, n0 + g * KC, n0 + at, a.N, raw);
-                if constexpr (KEEPS_LOW<T, EPI>)
-                    store_chunk(static_cast<T*>(a.low) + m * a.N, n0 + g * KC, n0 + at, a.N, low[g]);
+                store_chunk(y + m * a.ldy, n0 + g * KC, n0 + at, a.N, raw);
+                if constexpr (KEEPS_LOW<T, EPI>) store_chunk(y + a.N + m * a.ldy, n0 + g * KC, n0 + at, a.N, low[g]);
             }
         }
         auto put = [&](T* to) {
-            if (m - r + 16 <= a.rows) store_strip<T, VP, PO>(strip, to, m - r, a.rows, n0, a.N, lane, Flag<true>{});
-            else store_strip<T, VP, PO>(strip, to, m - r, a.rows, n0, a.N, lane, Flag<false>{});
+            const int64_t top = m - r;
+            if (top + 16 <= a.rows) store_strip<T, VP, PO>(strip, to, a.ldy, top, a.rows, n0, a.N, lane, Flag<true>{});
+            else store_strip<T, VP, PO>(strip, to, a.ldy, top, a.rows, n0, a.N, lane, Flag<false>{});
         };
         if (staged) {
             put(y);
             if constexpr (KEEPS_LOW<T, EPI>) {
 #pragma unroll
                 for (int g = 0; g < G; ++g) strip[r * PO + g * 4 + q] = low[g];
-                put(static_cast<T*>(a.low));
+                put(y + a.N);
             }
         }
     }
 }
 
-// The weights as the tile kernel takes them: fragments of W (or of W^T), 64
-// columns (4 tiles) after 64, within them chunk by chunk, zero past N and K, so
-// that a wavefront reads a fragment as 1 KB in a row.
+// The weights as the tile kernel takes them: fragments of W, or of W^T as often
+// beside itself as K holds its `inner` columns, 64 columns (4 tiles) after 64,
+// within them chunk by chunk, zero past N and K, so that a wavefront reads a
+// fragment as 1 KB in a row.
 template <class T, bool TRANSPOSED>
-__global__ __launch_bounds__(256) void pack_weights_kernel(const T* __restrict__ w, int N, int K, int chunks,
+__global__ __launch_bounds__(256) void pack_weights_kernel(const T* __restrict__ w, int N, int K, int inner, int chunks,
                                                            u32x4* __restrict__ out) {
     constexpr int E = VEC<T>;
     const int slot = blockIdx.x * 256 + threadIdx.x;
@@ -432,7 +437,7 @@ __global__ __launch_bounds__(256) void pack_weights_kernel(const T* __restrict__
         } else {
             float f[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) f[i] = k + i < K ? to_f32(w[(int64_t)(k + i) * N + n]) : 0.0f;
+            for (int i = 0; i < E; ++i) f[i] = k + i < K ? to_f32(w[(int64_t)((k + i) % inner) * N + n]) : 0.0f;
             v = pack<T>(f);
         }
     }
@@ -571,18 +576,18 @@ void linear_tile_kernel(LinearRows a) {
                 raw = linear_end<T, EPI, E>(a, z, raw, low[g]);
                 if (staged) slot = raw;
                 else if (whole.value || m < a.rows) {
-                    store_chunk(y + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
+                    store_chunk(y + m * a.ldy, n0 + g * KC, n0 + g * KC + q * E, a.N, raw);
                     if constexpr (KEEPS_LOW<T, EPI>)
-                        store_chunk(static_cast<T*>(a.low) + m * a.N, n0 + g * KC, n0 + g * KC + q * E, a.N, low[g]);
+                        store_chunk(y + a.N + m * a.ldy, n0 + g * KC, n0 + g * KC + q * E, a.N, low[g]);
                 }
             }
-            if (staged) store_strip<T, VP, PO>(mine, y, m0, a.rows, n0, a.N, lane, whole);
+            if (staged) store_strip<T, VP, PO>(mine, y, a.ldy, m0, a.rows, n0, a.N, lane, whole);
             else wave_fence();
             if constexpr (KEEPS_LOW<T, EPI>) {
                 if (staged) {
 #pragma unroll
                     for (int g = 0; g < G; ++g) mine[r * PO + g * 4 + q] = low[g];
-                    store_strip<T, VP, PO>(mine, static_cast<T*>(a.low), m0, a.rows, n0, a.N, lane, whole);
+                    store_strip<T, VP, PO>(mine, y + a.N, a.ldy, m0, a.rows, n0, a.N, lane, whole);
                 }
             }
         };
@@ -594,8 +599,10 @@ void linear_tile_kernel(LinearRows a) {
     }
 }
 
+// W^T, `times` beside itself.
 template <class T>
-__global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ w, int n, int k, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ w, int n, int k, int times,
+                                                        T* __restrict__ out) {
     __shared__ T tile[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     for (int i = ty; i < 32; i += 8) {
@@ -605,14 +612,15 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ w,
     __syncthreads();
     for (int i = ty; i < 32; i += 8) {
         const int row = blockIdx.x * 32 + i, col = blockIdx.y * 32 + tx;
-        if (row < k && col < n) out[(int64_t)row * n + col] = tile[tx][i];
+        if (row < k && col < n)
+            for (int j = 0; j < times; ++j) out[((int64_t)row * times + j) * n + col] = tile[tx][i];
     }
 }
 
 struct LinearGradW {
     Rows x;
     const void* dz;
-    const void* low;  // what dz leaves, rows x N, or NULL
+    bool split;       // a row of dz is N high halves, then N low ones
     int64_t ldz;
     int64_t rows, rows_per_split;
     int N, n_tiles, k_tiles, splits;
@@ -648,7 +656,7 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
     const int r = lane & 15, q = lane >> 4;
     const int wn = wave >> 1, wk = wave & 1;
     const bool sum_bias = kt == 0 && wk == 0;
-    const T* dz[2] = {static_cast<const T*>(a.dz), static_cast<const T*>(a.low)};
+    const T* dz = static_cast<const T*>(a.dz);
 
     u32x4 zr[PLANES][LZ];
     RowRaw<T, Q8> xr[LX];
@@ -658,7 +666,7 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
             const int u = i * 256 + tid;
             const int64_t m = m0 + u / CZ < end ? m0 + u / CZ : end - 1;
 #pragma unroll
-            for (int p = 0; p < PLANES; ++p) zr[p][i] = issue_row(dz[p] + m * a.ldz, n0 + u % CZ * E, a.N);
+            for (int p = 0; p < PLANES; ++p) zr[p][i] = issue_row(dz + m * a.ldz + p * a.N, n0 + u % CZ * E, a.N);
         }
 #pragma unroll
         for (int i = 0; i < LX; ++i) {
@@ -845,15 +853,16 @@ static void launch_long(const LinearRows& a, hipStream_t stream) {
     else launch_long_as<T, Q8, EPI, 2, 8, true>(a, stream);
 }
 // `packed`: room for the packed weights where the tile kernel takes the
-// product; TRANSPOSED: a.w is K x N.
+// product; TRANSPOSED: a.w is K / times x N.
 template <class T, bool Q8, int EPI, bool TRANSPOSED>
-static void launch_rows(LinearRows a, void* packed, hipStream_t stream) {
+static void launch_rows(LinearRows a, void* packed, hipStream_t stream, int times = 1) {
     if constexpr (sizeof(T) == 2) {
         if (tiled<T>(a.rows, a.K, a.N)) {
             const int64_t vectors = packed_vectors<T>(a.N, a.K);
             const int chunks = (a.K + CHUNK<T> - 1) / CHUNK<T>;
             hipLaunchKernelGGL((pack_weights_kernel<T, TRANSPOSED>), dim3((unsigned)(vectors / 256)), dim3(256), 0,
-                               stream, static_cast<const T*>(a.w), a.N, a.K, chunks, static_cast<u32x4*>(packed));
+                               stream, static_cast<const T*>(a.w), a.N, a.K, a.K / times, chunks,
+                               static_cast<u32x4*>(packed));
             a.w = packed;
             if (chunks <= 8) return launch_tile<T, Q8, EPI, 8>(a, stream);
             return launch_tile<T, Q8, EPI, 16>(a, stream);
@@ -861,8 +870,9 @@ static void launch_rows(LinearRows a, void* packed, hipStream_t stream) {
     }
     if constexpr (TRANSPOSED) {
         T* wt = static_cast<T*>(packed);
-        hipLaunchKernelGGL(transpose_kernel<T>, dim3((a.N + 31) / 32, (a.K + 31) / 32), dim3(256), 0, stream,
-                           static_cast<const T*>(a.w), a.K, a.N, wt);
+        const int inner = a.K / times;
+        hipLaunchKernelGGL(transpose_kernel<T>, dim3((a.N + 31) / 32, (inner + 31) / 32), dim3(256), 0, stream,
+                           static_cast<const T*>(a.w), inner, a.N, times, wt);
         a.w = wt;
     }
     switch (chunks_of<T>(a.K)) {
@@ -877,7 +887,7 @@ template <class T, bool Q8, int A, int B>
 static void launch_gradw_as(const LinearGradW& a, int splits, hipStream_t stream) {
     const dim3 grid((unsigned)(a.n_tiles * a.k_tiles * ((splits + 7) / 8 * 8)));
     if constexpr (SPLIT<T>) {
-        if (a.low) {
+        if (a.split) {
             hipLaunchKernelGGL((linear_gradw_kernel<T, Q8, A, B, 2>), grid, dim3(256), 0, stream, a);
             return;
         }
@@ -926,9 +936,9 @@ static BwdPlan bwd_plan(int64_t rows, int K, int N) {
 static size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Scratch of the backward pass: the splits' dW and db; unless it is fused also
-// dz, in two planes where it is split, and W^T.
+// dz, its rows twice as long where it is split, and W^T, as often.
 struct BwdScratch {
-    size_t part, dz, low, wt, total;
+    size_t part, dz, wt, total;
 };
 template <class T>
 static BwdScratch bwd_scratch(int64_t rows, int K, int N) {
@@ -936,13 +946,11 @@ static BwdScratch bwd_scratch(int64_t rows, int K, int N) {
     BwdScratch s;
     s.part = 0;
     s.dz = aligned((size_t)p.splits * ((size_t)N * K + N) * 4);
-    const size_t plane = p.fused ? 0 : aligned((size_t)rows * N * sizeof(T));
-    s.low = s.dz + plane;
-    s.wt = s.low + (SPLIT<T> ? plane : 0);
+    const int halves = SPLIT<T> ? 2 : 1;
+    s.wt = s.dz + (p.fused ? 0 : aligned((size_t)rows * N * halves * sizeof(T)));
     // W^T as it is, or packed; W packed in its place before.
-    const size_t packed = (size_t)(packed_vectors<T>(N, K) > packed_vectors<T>(K, N) ? packed_vectors<T>(N, K)
-                                                                                       : packed_vectors<T>(K, N)) * 16;
-    s.total = s.wt + (p.fused ? 0 : aligned(packed));
+    const int64_t forward = packed_vectors<T>(N, K), back = packed_vectors<T>(K, N * halves);
+    s.total = s.wt + (p.fused ? 0 : aligned((size_t)(forward > back ? forward : back) * 16));
     return s;
 }
 
@@ -956,7 +964,7 @@ static int linear_fwd(const gs3d_linear_args& g, void* scratch, hipStream_t stre
     LinearRows a{};
     a.x = Rows{g.x, g.x_stride, {}, g.inner};
     a.w = g.weight, a.bias = g.bias, a.other = g.residual, a.ldo = g.residual_stride, a.y = g.y;
-    a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
+    a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.ldy = g.outer, a.act = g.activation;
     // The stream kernel keeps the rows as it reads them.
     if (g.codes && !few_rows(a) && chunks_of<T>(a.K) <= 4) a.keep_codes = g.codes, a.keep_scales = g.scales;
     else if (g.codes) quantize_rows(g.x, g.x_stride, g.rows, g.inner, g.dtype, g.codes, g.scales, stream);
@@ -985,27 +993,26 @@ static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t 
             fused_launch<T>(a, Q8, p.splits, stream);
         }
     } else {
-        const void *dz = g.upstream, *low = nullptr;
+        const void* dz = g.upstream;
         int64_t ldz = g.upstream_stride;
+        const int halves = SPLIT<T> && g.activation != GS3D_ACT_NONE ? 2 : 1;  // of dz
         if (g.activation != GS3D_ACT_NONE && g.rows > 0) {
             LinearRows a{};
             a.x = x, a.w = g.weight, a.bias = g.bias, a.other = g.upstream, a.ldo = g.upstream_stride;
-            a.y = scratch + at.dz, a.low = scratch + at.low;
+            a.y = scratch + at.dz, a.ldy = (int64_t)halves * g.outer;
             a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.act = g.activation;
             launch_rows<T, Q8, 1, false>(a, scratch + at.wt, stream);
-            dz = scratch + at.dz;
-            if (SPLIT<T>) low = scratch + at.low;
-            ldz = g.outer;
+            dz = a.y, ldz = a.ldy;
         }
         if (g.grad_x && g.rows > 0) {
             LinearRows a{};
-            a.x = Rows{dz, ldz, {}, g.outer}, a.w = g.weight, a.y = g.grad_x;
-            a.rows = g.rows, a.K = g.outer, a.N = g.inner, a.act = GS3D_ACT_NONE;
-            launch_rows<T, false, 0, true>(a, scratch + at.wt, stream);
+            a.x = Rows{dz, ldz, {}, halves * g.outer}, a.w = g.weight, a.y = g.grad_x, a.ldy = g.inner;
+            a.rows = g.rows, a.K = halves * g.outer, a.N = g.inner, a.act = GS3D_ACT_NONE;
+            launch_rows<T, false, 0, true>(a, scratch + at.wt, stream, halves);
         }
         if (params) {
-            LinearGradW a{x, dz, low, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, p.splits, part,
-                          g.inner};
+            LinearGradW a{x, dz, halves == 2, ldz, g.rows, p.rows_per_split, g.outer, p.n_tiles, p.k_tiles, p.splits,
+                          part, g.inner};
             launch_gradw<T, Q8>(a, p.splits, stream);
         }
     }

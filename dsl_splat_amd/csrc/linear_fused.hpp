@@ -224,11 +224,16 @@ void linear_bwd_fused_kernel(LinearFused a) {
 #pragma unroll
                     for (int g = 0; g < NCH; ++g) {
                         if (SKIP && g * KC >= a.N) break;
-                        const u32x4 dz = z_lds[0][(strip + r) * PN + g * 4 + q];
+                        u32x4 dz[PLANES];
 #pragma unroll
-                        for (int t = 0; t < TG; ++t)
-                            out[t] = multiply_chunk<T>(read_transposed<T, true>(w_lds, PK, g * KC, c * TG + t, lane),
-                                                       dz, out[t], a.N - g * KC);
+                        for (int p = 0; p < PLANES; ++p) dz[p] = z_lds[p][(strip + r) * PN + g * 4 + q];
+#pragma unroll
+                        for (int t = 0; t < TG; ++t) {
+                            const u32x4 wf = read_transposed<T, true>(w_lds, PK, g * KC, c * TG + t, lane);
+#pragma unroll
+                            for (int p = 0; p < PLANES; ++p)
+                                out[t] = multiply_chunk<T>(wf, dz[p], out[t], a.N - g * KC);
+                        }
                     }
                     settle(out);
                     float v[E];

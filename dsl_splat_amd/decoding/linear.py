@@ -97,8 +97,8 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation:
     Products are summed in 32 bits and rounded once.  ``activation`` is "none",
     "relu", "silu" or "gelu" (the exact one, z Phi(z)).  Differentiable in
     every tensor; the backward pass computes the activation's argument again
-    rather than keep it, and takes the gradient at it to the dtype's precision
-    for x's gradient and to twice that for the weight's and the bias's.  With checkpoint="int8" the input is kept in 8 bits
+    rather than keep it, and takes the gradient at it to twice the dtype's
+    precision.  With checkpoint="int8" the input is kept in 8 bits
     (``quantize_activations``) and the gradients are those at the kept value.
     """
     check_input("x", x, 1)
