@@ -464,9 +464,22 @@ GS3D_DEV int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
 template <class T>
 constexpr bool SPLIT = sizeof(T) == 2;
 
-// The vector's high halves; v keeps what they leave, nothing beside an infinity.
+// The vector's high halves; v keeps what they leave.  A slope (1.13 at most)
+// can take a float16 gradient past the type's range: the high half then is its
+// largest value and the low one has the rest, which of an infinity or a NaN is
+// itself.  bfloat16's high half is infinite with its value, the low one zero.
 template <class T>
 GS3D_DEV u32x4 take_high(float (&v)[VEC<T>]) {
+    if constexpr (__is_same(T, f16_t)) {
+        float top[VEC<T>], h[VEC<T>];
+#pragma unroll
+        for (int i = 0; i < VEC<T>; ++i) top[i] = __builtin_amdgcn_fmed3f(v[i], -65504.0f, 65504.0f);
+        const u32x4 high = pack<T>(top);
+        unpack<T>(high, h);
+#pragma unroll
+        for (int i = 0; i < VEC<T>; ++i) v[i] -= h[i];
+        return high;
+    }
     const u32x4 high = pack<T>(v);
     float h[VEC<T>];
     unpack<T>(high, h);

@@ -37,3 +37,23 @@ def test_input_gradients_err_by_their_own_rounding(rows, inner, outer, dtype):
         want = ref.linear_grads(seen, w, b, up, kind)["x"][0]
         least = (want.to(dtype).double() - want).norm()
         assert (got.double() - want).norm() <= 1.02 * least, (kind, ((got.double() - want).norm() / least).item())
+
+
+@pytest.mark.parametrize("inner,outer", [(40, 72), (300, 140)])
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+def test_gradients_beyond_the_range_of_float16(kind, inner, outer):
+    """A slope above one takes an upstream gradient near float16's largest value
+    past it, on the way to results that are well inside."""
+    print("linear", kind, inner, outer, flush=True)
+    g = torch.Generator().manual_seed(5)
+    x = _normal(g, 1200, inner, dtype=torch.float16)
+    w = _normal(g, outer, inner, scale=0.01 * inner ** -0.5, dtype=torch.float16)
+    b = torch.full((outer,), {"silu": 2.4, "gelu": 1.4}[kind], dtype=torch.float16, device=DEV)  # where the slope is largest
+    up = torch.zeros((1200, outer), dtype=torch.float16, device=DEV)
+    up[5, 3], up[5, 4], up[700, 9] = 65504.0, -65504.0, 65504.0
+    x[5], x[700] = x[5] * 2 ** -5, x[700] * 2 ** -5
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    got = torch.autograd.grad(decoding.linear(*leaves, b, activation=kind), leaves, up)
+    grads = ref.linear_grads(x.detach(), w.detach(), b, up, kind)
+    for name, value in zip(("x", "weight"), got):
+        ref.check(name, value, *grads[name])
