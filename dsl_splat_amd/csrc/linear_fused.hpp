@@ -139,7 +139,8 @@ void linear_bwd_fused_kernel(LinearFused a) {
             yr[i] = issue_row<T, WIDE>(dy + m * a.ldy, u % DN * E, a.N);
         }
     };
-    // Rows past the end add nothing, whatever the last row holds.
+    // Rows past the end add nothing, whatever the last row holds (dz is cleared
+    // again after the slope, which an infinite weight makes NaN there).
     auto fill = [&](int64_t m0) {
         const u32x4 zero = {0u, 0u, 0u, 0u};
         const bool whole = m0 + ROWS <= end;
@@ -198,6 +199,14 @@ void linear_bwd_fused_kernel(LinearFused a) {
 #pragma unroll
                     for (int i = 0; i < E; ++i) arg[i] = z[i / 4][i & 3];
                     pull_back(grad, arg, a.act);
+                    // Past N and past the last row an infinity of x or of W
+                    // meets a zero, and the slope there is NaN.
+                    if (g * KC + KC > a.N || m0 + ROWS > end) {
+                        const bool live = m0 + strip + r < end;
+#pragma unroll
+                        for (int i = 0; i < E; ++i)
+                            grad[i] = live && g * KC + q * E + i < a.N ? grad[i] : 0.0f;
+                    }
                     if constexpr (PLANES == 2) {
                         z_lds[0][at] = take_high<T>(grad);
                         z_lds[1][at] = pack<T>(grad);

@@ -1,0 +1,60 @@
+"""The decoder at the edges of its arguments."""
+
+import math
+
+import pytest
+import torch
+
+import decoding_reference as ref
+from dsl_splat_amd import decoding
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _case(rows, inner, outer, dtype):
+    g = torch.Generator().manual_seed(rows + inner + outer)
+    normal = lambda *shape, scale=1.0: (torch.randn(shape, generator=g) * scale).to(dtype).to(DEV)
+    return normal(rows, inner), normal(outer, inner, scale=inner ** -0.5), normal(outer, scale=0.3), normal(rows, outer)
+
+
+def _same(name, got, want, bound):
+    """Within the bound where the formula is finite, else the formula's value."""
+    got = got.double()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine), name
+    assert torch.equal(got[~fine].isnan(), want[~fine].isnan()), name
+    assert ((got - want).abs()[fine] <= bound[fine]).all(), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,inner,outer", [(300, 33, 97), (133, 40, 72), (130, 16, 5), (257, 64, 64), (200, 300, 140)])
+@pytest.mark.parametrize("checkpoint", (None, "int8"))
+def test_relu_of_infinite_arguments(checkpoint, rows, inner, outer, dtype):
+    """relu's slope is 1 or 0 at an infinity, so gradients stay what the formula
+    gives, whether or not the channels and rows fill the kernels' tiles."""
+    print("linear", rows, inner, outer, dtype, checkpoint, flush=True)
+    x, w, b, up = _case(rows, inner, outer, dtype)
+    if checkpoint is None:  # (in 8 bits the block reads back as NaN)
+        x[7, 3], x[rows - 1, 0] = math.inf, -math.inf
+        clean = ref.linear_grads(torch.where(torch.isfinite(x), x, torch.zeros_like(x)), w, b, up, "relu")["x"][1]
+        leaf = x.detach().requires_grad_(True)
+        (dx,) = torch.autograd.grad(decoding.linear(leaf, w, b, activation="relu"), leaf, up)
+        z = x.double() @ w.double().T + b.double()
+        dz = up.double() * (z > 0)
+        bound = clean.amax() + (outer + 2) * (ref.U + ref.UNIT[dtype]) * (dz.abs() @ w.double().abs())
+        _same("dx", dx, dz @ w.double(), bound)
+    # An infinite weight: z is infinite in every row but only of its channel.
+    x = torch.where(torch.isfinite(x), x, torch.ones_like(x))
+    w = w.clone()
+    w[2, 1] = math.inf
+    leaf = w.detach().requires_grad_(True)
+    (dw,) = torch.autograd.grad(decoding.linear(x, leaf, b, activation="relu", checkpoint=checkpoint), leaf, up)
+    seen = (ref.kept(x) if checkpoint else x).double()
+    z = seen @ w.double().T + b.double()
+    dz = up.double() * torch.where(z.isnan(), z, (z > 0).double())
+    near = up.double().abs() * (z.abs() <= (inner + 2) * ref.U * (seen.abs() @ torch.where(torch.isfinite(w), w, 0 * b[:, None]).double().abs().T + b.double().abs()))
+    bound = near.T @ seen.abs() + ((rows + 2) * ref.U + ref.UNIT[dtype]) * (dz.abs().T @ seen.abs()) + ref.TINY[dtype]
+    _same("dw", dw, dz.T @ seen, bound)
