@@ -986,17 +986,17 @@ static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t 
     const bool params = g.grad_weight || g.grad_bias;
     float* part = reinterpret_cast<float*>(scratch + at.part);
     int splits = p.splits;
-    if (p.fused) {
-        if (g.rows > 0 || params) {
-            LinearFused a{x, g.weight, g.bias, g.upstream, g.upstream_stride, g.grad_x, params ? part : nullptr,
-                          g.rows, p.rows_per_split, g.inner, g.outer, g.activation, &splits};
-            fused_launch<T>(a, Q8, p.splits, stream);
-        }
+    if (g.rows == 0) {
+        splits = 0;  // the parameters' gradients are sums of nothing, and no tensor has to be there
+    } else if (p.fused) {
+        LinearFused a{x, g.weight, g.bias, g.upstream, g.upstream_stride, g.grad_x, params ? part : nullptr,
+                      g.rows, p.rows_per_split, g.inner, g.outer, g.activation, &splits};
+        fused_launch<T>(a, Q8, p.splits, stream);
     } else {
         const void* dz = g.upstream;
         int64_t ldz = g.upstream_stride;
         const int halves = SPLIT<T> && g.activation != GS3D_ACT_NONE ? 2 : 1;  // of dz
-        if (g.activation != GS3D_ACT_NONE && g.rows > 0) {
+        if (g.activation != GS3D_ACT_NONE) {
             LinearRows a{};
             a.x = x, a.w = g.weight, a.bias = g.bias, a.other = g.upstream, a.ldo = g.upstream_stride;
             a.y = scratch + at.dz, a.ldy = (int64_t)halves * g.outer;
@@ -1004,7 +1004,7 @@ static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t 
             launch_rows<T, Q8, 1, false>(a, scratch + at.wt, stream);
             dz = a.y, ldz = a.ldy;
         }
-        if (g.grad_x && g.rows > 0) {
+        if (g.grad_x) {
             LinearRows a{};
             a.x = Rows{dz, ldz, {}, halves * g.outer}, a.w = g.weight, a.y = g.grad_x, a.ldy = g.inner;
             a.rows = g.rows, a.K = halves * g.outer, a.N = g.inner, a.act = GS3D_ACT_NONE;

@@ -583,8 +583,9 @@ int gs3d_linear_fwd(const gs3d_linear_args* args, void* scratch, size_t scratch_
 /* Gradients of gs3d_linear_fwd from upstream = dL/dy (the residual's gradient
  * is upstream itself): with z = x W^T + bias and dz = upstream act'(z), z
  * computed again, grad_x = dz W, grad_weight = dz^T x, grad_bias = sum dz;
- * each may be NULL.  The input is either x or, in 8 bits, codes and scales
- * (gs3d_quantize_activations; x NULL then), which stand for x everywhere.
+ * each may be NULL.  Without rows grad_weight and grad_bias are zeroed and no
+ * tensor has to be there.  The input is either x or, in 8 bits, codes and
+ * scales (gs3d_quantize_activations; x NULL then), which stand for x everywhere.
  * Scratch: gs3d_linear_bwd_scratch_bytes, 16-byte aligned. */
 typedef struct gs3d_linear_bwd_args {
     int64_t rows;

@@ -1,5 +1,6 @@
 """The decoder at the edges of its arguments."""
 
+import ctypes
 import math
 
 import pytest
@@ -7,6 +8,7 @@ import torch
 
 import decoding_reference as ref
 from dsl_splat_amd import decoding
+from dsl_splat_amd.runtime import abi, native
 
 pytestmark = pytest.mark.gpu
 
@@ -55,6 +57,19 @@ def test_relu_of_infinite_arguments(checkpoint, rows, inner, outer, dtype):
     seen = (ref.kept(x) if checkpoint else x).double()
     z = seen @ w.double().T + b.double()
     dz = up.double() * torch.where(z.isnan(), z, (z > 0).double())
-    near = up.double().abs() * (z.abs() <= (inner + 2) * ref.U * (seen.abs() @ torch.where(torch.isfinite(w), w, 0 * b[:, None]).double().abs().T + b.double().abs()))
+    size = seen.abs() @ torch.where(torch.isfinite(w), w, 0 * b[:, None]).double().abs().T + b.double().abs()
+    near = up.double().abs() * (z.abs() <= (inner + 2) * ref.U * size)
     bound = near.T @ seen.abs() + ((rows + 2) * ref.U + ref.UNIT[dtype]) * (dz.abs().T @ seen.abs()) + ref.TINY[dtype]
     _same("dw", dw, dz.T @ seen, bound)
+
+
+def test_no_pixels_at_the_c_entry_of_the_product():
+    """Sums over no rows are zero; nothing is read for them."""
+    dw, db = torch.ones(6 * 8, device=DEV), torch.ones(6, device=DEV)
+    a = abi.LinearBwdArgs()
+    a.rows, a.inner, a.outer, a.grad_weight, a.grad_bias = 0, 8, 6, native.ptr(dw), native.ptr(db)
+    work = torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
+    stream = native.stream(torch.device(DEV, 0))
+    native.call("gs3d_linear_bwd", ctypes.byref(a), native.ptr(work), work.numel(), stream)
+    torch.cuda.synchronize()
+    assert not dw.any() and not db.any()
