@@ -476,6 +476,14 @@ static int norm_fwd(const gs3d_group_norm_args& g, void* scratch, hipStream_t st
     return launch_status("gs3d_group_norm_fwd");
 }
 
+// The images' sums to dgamma and dbeta (zero without images).
+template <class T>
+static void launch_params(const gs3d_group_norm_bwd_args& g, int images, const float2* sums, hipStream_t stream) {
+    if (g.grad_weight || g.grad_bias)
+        hipLaunchKernelGGL(norm_params_kernel<T>, dim3(blocks_for(g.channels, 256)), dim3(256), 0, stream, images,
+                           g.channels, sums, static_cast<T*>(g.grad_weight), static_cast<T*>(g.grad_bias));
+}
+
 template <class T, bool Q8, bool WIDE>
 static int norm_bwd_as(const gs3d_group_norm_bwd_args& g, char* scratch, hipStream_t stream) {
     NormShape s = norm_shape(g.images, g.pixels, g.channels, g.groups, g.dtype);
@@ -495,13 +503,15 @@ static int norm_bwd_as(const gs3d_group_norm_bwd_args& g, char* scratch, hipStre
     if (g.grad_x)
         hipLaunchKernelGGL((norm_grad_kernel<T, Q8, WIDE>), grid, dim3(256), 0, stream, s, a, p, dy, g.upstream_stride,
                            pulls, static_cast<T*>(g.grad_x));
-    if (g.grad_weight || g.grad_bias)
-        hipLaunchKernelGGL(norm_params_kernel<T>, dim3(blocks_for(s.channels, 256)), dim3(256), 0, stream, g.images,
-                           s.channels, sums, static_cast<T*>(g.grad_weight), static_cast<T*>(g.grad_bias));
+    launch_params<T>(g, g.images, sums, stream);
     return launch_status("gs3d_group_norm_bwd");
 }
 template <class T, bool Q8>
 static int norm_bwd(const gs3d_group_norm_bwd_args& g, char* scratch, hipStream_t stream) {
+    if (g.images == 0 || g.pixels == 0) {  // the parameters' gradients are sums of nothing
+        launch_params<T>(g, 0, nullptr, stream);
+        return launch_status("gs3d_group_norm_bwd");
+    }
     return g.channels >= VEC<T> ? norm_bwd_as<T, Q8, true>(g, scratch, stream)
                                 : norm_bwd_as<T, Q8, false>(g, scratch, stream);
 }
@@ -543,13 +553,13 @@ extern "C" int gs3d_group_norm_bwd(const gs3d_group_norm_bwd_args* g, void* scra
         return GS3D_ERR_ARGUMENT;
     const bool q8 = g->codes != nullptr;
     if (q8 != (g->scales != nullptr) || (q8 && g->x)) return GS3D_ERR_ARGUMENT;
-    if (g->images == 0 || g->pixels == 0) return GS3D_OK;
-    if (!g->statistics || !g->upstream || g->upstream_stride < g->channels ||
-        (!q8 && (!g->x || g->x_stride < g->channels)))
-        return GS3D_ERR_ARGUMENT;
-    if (!scratch ||
-        scratch_bytes < gs3d_group_norm_scratch_bytes(g->images, g->pixels, g->channels, g->groups, g->dtype))
-        return GS3D_ERR_SCRATCH;
+    const size_t needed = gs3d_group_norm_scratch_bytes(g->images, g->pixels, g->channels, g->groups, g->dtype);
+    if (needed > 0) {  // there are pixels
+        if (!g->statistics || !g->upstream || g->upstream_stride < g->channels ||
+            (!q8 && (!g->x || g->x_stride < g->channels)))
+            return GS3D_ERR_ARGUMENT;
+        if (!scratch || scratch_bytes < needed) return GS3D_ERR_SCRATCH;
+    }
     const hipStream_t s = gs3d::as_stream(stream);
     char* p = static_cast<char*>(scratch);
     if (g->dtype == GS3D_F32) return q8 ? gs3d::norm_bwd<float, true>(*g, p, s) : gs3d::norm_bwd<float, false>(*g, p, s);

@@ -69,22 +69,17 @@ class _GroupNorm(torch.autograd.Function):
         upstream, stride = rows_of(gradient)
         grads = [torch.empty(shape, dtype=gradient.dtype, device=gradient.device) if needed else None
                  for shape, needed in zip((ctx.shape, (channels,), (channels,)), ctx.needs_input_grad)]
-        if gradient.numel():
-            a = abi.GroupNormBwdArgs()
-            a.images, a.pixels = math.prod(ctx.shape[:-3]), ctx.shape[-3] * ctx.shape[-2]
-            a.channels, a.groups = channels, ctx.groups
-            a.dtype, a.activation = DTYPES[gradient.dtype], ctx.activation
-            a.x, a.x_stride = native.ptr(x), ctx.x_stride
-            a.codes, a.scales = native.ptr(codes), native.ptr(scales)
-            a.weight, a.bias, a.statistics = native.ptr(weight), native.ptr(bias), native.ptr(statistics)
-            a.upstream, a.upstream_stride = native.ptr(upstream), stride
-            a.grad_x, a.grad_weight, a.grad_bias = (native.ptr(g) for g in grads)
-            work = _scratch(ctx.shape, ctx.groups, a.dtype, gradient.device)
-            launch("gs3d_group_norm_bwd", ctypes.byref(a), gradient.device, native.ptr(work), work.numel())
-        else:
-            for g in grads:
-                if g is not None:
-                    g.zero_()
+        a = abi.GroupNormBwdArgs()
+        a.images, a.pixels = math.prod(ctx.shape[:-3]), ctx.shape[-3] * ctx.shape[-2]
+        a.channels, a.groups = channels, ctx.groups
+        a.dtype, a.activation = DTYPES[gradient.dtype], ctx.activation
+        a.x, a.x_stride = native.ptr(x), ctx.x_stride
+        a.codes, a.scales = native.ptr(codes), native.ptr(scales)
+        a.weight, a.bias, a.statistics = native.ptr(weight), native.ptr(bias), native.ptr(statistics)
+        a.upstream, a.upstream_stride = native.ptr(upstream), stride
+        a.grad_x, a.grad_weight, a.grad_bias = (native.ptr(g) for g in grads)
+        work = _scratch(ctx.shape, ctx.groups, a.dtype, gradient.device)
+        launch("gs3d_group_norm_bwd", ctypes.byref(a), gradient.device, native.ptr(work), work.numel())
         return (*grads, None, None, None, None)
 
 

@@ -634,7 +634,8 @@ int gs3d_group_norm_fwd(const gs3d_group_norm_args* args, void* scratch, size_t 
 
 /* Gradients of gs3d_group_norm_fwd; x or codes and scales as in
  * gs3d_linear_bwd (the statistics stay those of x).  Any gradient may be
- * NULL. */
+ * NULL.  Without pixels grad_weight and grad_bias are zeroed and no tensor has
+ * to be there. */
 typedef struct gs3d_group_norm_bwd_args {
     int32_t images;
     int64_t pixels;

@@ -73,3 +73,14 @@ def test_no_pixels_at_the_c_entry_of_the_product():
     native.call("gs3d_linear_bwd", ctypes.byref(a), native.ptr(work), work.numel(), stream)
     torch.cuda.synchronize()
     assert not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("images,pixels", [(0, 5), (3, 0)])
+def test_no_pixels_at_the_c_entry_of_the_norm(images, pixels):
+    dw, db = torch.ones(8, device=DEV), torch.ones(8, device=DEV)
+    a = abi.GroupNormBwdArgs()
+    a.images, a.pixels, a.channels, a.groups = images, pixels, 8, 4
+    a.grad_weight, a.grad_bias = native.ptr(dw), native.ptr(db)
+    native.call("gs3d_group_norm_bwd", ctypes.byref(a), None, 0, native.stream(torch.device(DEV, 0)))
+    torch.cuda.synchronize()
+    assert not dw.any() and not db.any()
