@@ -26,18 +26,32 @@ class QuantizedActivations:
     @native.no_grad
     def dequantize(self) -> Tensor:
         """The values that were kept, in the dtype that was quantised."""
-        out = torch.empty(self.codes.shape, dtype=self.dtype, device=self.codes.device)
-        channels = self.codes.shape[-1]
+        codes, scales = self.codes, self.scales
+        if not (isinstance(codes, Tensor) and codes.is_cuda and codes.dtype == torch.int8 and codes.ndim):
+            raise ValueError("codes must be a CUDA int8 tensor of at least one dimension")
+        if not (isinstance(scales, Tensor) and scales.device == codes.device and scales.dtype == torch.uint8):
+            raise ValueError(f"scales must be uint8 on {codes.device}")
+        channels = codes.shape[-1]
+        if channels < 1 or tuple(scales.shape) != _scales_shape(codes.shape):
+            raise ValueError(f"codes {tuple(codes.shape)} need a channel and scales {_scales_shape(codes.shape)}, got "
+                             f"{tuple(scales.shape)}")
+        if self.dtype not in DTYPES:
+            raise ValueError(f"dtype must be one of {tuple(DTYPES)}, got {self.dtype}")
+        out = torch.empty(codes.shape, dtype=self.dtype, device=codes.device)
         if out.numel():
-            launch("gs3d_dequantize_activations", native.ptr(self.codes), out.device, native.ptr(self.scales),
+            codes, scales = codes.contiguous(), scales.contiguous()
+            launch("gs3d_dequantize_activations", native.ptr(codes), out.device, native.ptr(scales),
                    out.numel() // channels, channels, DTYPES[self.dtype], native.ptr(out))
         return out
 
 
+def _scales_shape(shape) -> tuple[int, ...]:
+    return (*shape[:-1], (shape[-1] + BLOCK - 1) // BLOCK)
+
+
 def empty_quantized(x: Tensor) -> QuantizedActivations:
-    channels = x.shape[-1]
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(x.shape[:-1] + ((channels + BLOCK - 1) // BLOCK,), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_scales_shape(x.shape), dtype=torch.uint8, device=x.device)
     return QuantizedActivations(codes, scales, x.dtype)
 
 

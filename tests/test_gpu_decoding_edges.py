@@ -84,3 +84,18 @@ def test_no_pixels_at_the_c_entry_of_the_norm(images, pixels):
     native.call("gs3d_group_norm_bwd", ctypes.byref(a), None, 0, native.stream(torch.device(DEV, 0)))
     torch.cuda.synchronize()
     assert not dw.any() and not db.any()
+
+
+def test_quantized_values_of_any_layout():
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn((40, 64), generator=g).to(DEV)
+    q = decoding.quantize_activations(x)
+    part = decoding.QuantizedActivations(q.codes[::2], q.scales[::2], q.dtype)
+    assert torch.equal(part.dequantize(), q.dequantize()[::2])
+    bad = [(q.codes.int(), q.scales, q.dtype), (q.codes, q.scales.int(), q.dtype), (q.codes, q.scales[:-1], q.dtype),
+           (q.codes, q.scales[:, :1], q.dtype), (q.codes.cpu(), q.scales, q.dtype), (q.codes, q.scales.cpu(), q.dtype),
+           (q.codes, q.scales, torch.float64), (q.codes[:, :0], q.scales[:, :0], q.dtype)]
+    for i, args in enumerate(bad):
+        with pytest.raises(ValueError):
+            decoding.QuantizedActivations(*args).dequantize()
+            pytest.fail(f"case {i} was accepted")
