@@ -935,21 +935,23 @@ static BwdPlan bwd_plan(int64_t rows, int K, int N) {
 
 static size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// Scratch of the backward pass: the splits' dW and db; unless it is fused also
-// dz, its rows twice as long where it is split, and W^T, as often.
+// Scratch of the backward pass of a call that wants dW or db (params) and dx,
+// of a product that ends in an activation or not: the splits' dW and db; unless
+// it is fused also dz, its rows twice as long where it is split, and W^T, as
+// often.  Without an activation dz is the upstream gradient itself.
 struct BwdScratch {
     size_t part, dz, wt, total;
 };
 template <class T>
-static BwdScratch bwd_scratch(int64_t rows, int K, int N) {
+static BwdScratch bwd_scratch(int64_t rows, int K, int N, bool act, bool params, bool dx) {
     const BwdPlan p = bwd_plan<T>(rows, K, N);
     BwdScratch s;
     s.part = 0;
-    s.dz = aligned((size_t)p.splits * ((size_t)N * K + N) * 4);
-    const int halves = SPLIT<T> ? 2 : 1;
-    s.wt = s.dz + (p.fused ? 0 : aligned((size_t)rows * N * halves * sizeof(T)));
+    s.dz = params ? aligned((size_t)p.splits * ((size_t)N * K + N) * 4) : 0;
+    const int halves = SPLIT<T> && act ? 2 : 1;
+    s.wt = s.dz + (act && !p.fused ? aligned((size_t)rows * N * halves * sizeof(T)) : 0);
     // W^T as it is, or packed; W packed in its place before.
-    const int64_t forward = packed_vectors<T>(N, K), back = packed_vectors<T>(K, N * halves);
+    const int64_t forward = act ? packed_vectors<T>(N, K) : 0, back = dx ? packed_vectors<T>(K, N * halves) : 0;
     s.total = s.wt + (p.fused ? 0 : aligned((size_t)(forward > back ? forward : back) * 16));
     return s;
 }
@@ -976,14 +978,15 @@ static int linear_fwd(const gs3d_linear_args& g, void* scratch, hipStream_t stre
 template <class T, bool Q8>
 static int linear_bwd(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t stream) {
     const BwdPlan p = bwd_plan<T>(g.rows, g.inner, g.outer);
-    const BwdScratch at = bwd_scratch<T>(g.rows, g.inner, g.outer);
+    const bool params = g.grad_weight || g.grad_bias;
+    const BwdScratch at =
+        bwd_scratch<T>(g.rows, g.inner, g.outer, g.activation != GS3D_ACT_NONE, params, g.grad_x != nullptr);
     // Without an activation only dW sees the input.  Where neither is wanted the
     // caller may not have it: a row of the weights then stands in for every
     // row, and the dW that comes of it is dropped.
     const bool seen = g.grad_weight || g.activation != GS3D_ACT_NONE;
     if (!seen && Q8) return linear_bwd<T, false>(g, scratch, stream);
     const Rows x{seen ? g.x : g.weight, seen ? g.x_stride : 0, {g.codes, g.scales, g.inner}, g.inner};
-    const bool params = g.grad_weight || g.grad_bias;
     float* part = reinterpret_cast<float*>(scratch + at.part);
     int splits = p.splits;
     if (g.rows == 0) {

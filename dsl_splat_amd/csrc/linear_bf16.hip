@@ -13,6 +13,8 @@ int linear_bwd_bf16(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t st
     return g.codes ? linear_bwd<bf16_t, true>(g, scratch, stream) : linear_bwd<bf16_t, false>(g, scratch, stream);
 }
 
-size_t linear_bwd_bytes_bf16(int64_t rows, int K, int N) { return bwd_scratch<bf16_t>(rows, K, N).total; }
+size_t linear_bwd_bytes_bf16(int64_t rows, int K, int N, bool act, bool params, bool dx) {
+    return bwd_scratch<bf16_t>(rows, K, N, act, params, dx).total;
+}
 
 }  // namespace gs3d

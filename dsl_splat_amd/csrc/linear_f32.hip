@@ -13,6 +13,8 @@ int linear_bwd_f32(const gs3d_linear_bwd_args& g, char* scratch, hipStream_t str
     return g.codes ? linear_bwd<float, true>(g, scratch, stream) : linear_bwd<float, false>(g, scratch, stream);
 }
 
-size_t linear_bwd_bytes_f32(int64_t rows, int K, int N) { return bwd_scratch<float>(rows, K, N).total; }
+size_t linear_bwd_bytes_f32(int64_t rows, int K, int N, bool act, bool params, bool dx) {
+    return bwd_scratch<float>(rows, K, N, act, params, dx).total;
+}
 
 }  // namespace gs3d

@@ -82,9 +82,9 @@ class _Linear(torch.autograd.Function):
             a.weight, a.bias = native.ptr(weight), native.ptr(bias)
             a.upstream, a.upstream_stride = native.ptr(upstream), stride
             a.grad_x, a.grad_weight, a.grad_bias = (native.ptr(g) for g in grads[:3])
-            nbytes = native.query("gs3d_linear_bwd_scratch_bytes", a.rows, inner, outer, a.dtype)
-            work = scratch(nbytes, weight.device)
-            launch("gs3d_linear_bwd", ctypes.byref(a), weight.device, native.ptr(work), work.numel())
+            nbytes = native.query("gs3d_linear_bwd_call_scratch_bytes", ctypes.byref(a))
+            work = scratch(nbytes, weight.device) if nbytes else None
+            launch("gs3d_linear_bwd", ctypes.byref(a), weight.device, native.ptr(work), nbytes)
         return (*grads, None, None)
 
 

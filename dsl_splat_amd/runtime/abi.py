@@ -9,7 +9,7 @@ import ctypes
 c_float_p = ctypes.POINTER(ctypes.c_float)
 c_int32_p = ctypes.POINTER(ctypes.c_int32)
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 # Tile modes (GS3D_TILE_*), named as the reference's TileMode literals.
 TILE_MODES = {"radius": 0, "snugbox": 1, "accutile": 2}
@@ -404,6 +404,7 @@ FUNCTIONS = {
     "gs3d_linear_fwd_scratch_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
     "gs3d_linear_fwd": (ctypes.c_int, [ctypes.POINTER(LinearArgs), _P, _SZ, _P]),
     "gs3d_linear_bwd_scratch_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
+    "gs3d_linear_bwd_call_scratch_bytes": (_SZ, [ctypes.POINTER(LinearBwdArgs)]),
     "gs3d_linear_bwd": (ctypes.c_int, [ctypes.POINTER(LinearBwdArgs), _P, _SZ, _P]),
     "gs3d_group_norm_scratch_bytes": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
     "gs3d_group_norm_fwd": (ctypes.c_int, [ctypes.POINTER(GroupNormArgs), _P, _SZ, _P]),

@@ -586,7 +586,10 @@ int gs3d_linear_fwd(const gs3d_linear_args* args, void* scratch, size_t scratch_
  * each may be NULL.  Without rows grad_weight and grad_bias are zeroed and no
  * tensor has to be there.  The input is either x or, in 8 bits, codes and
  * scales (gs3d_quantize_activations; x NULL then), which stand for x everywhere.
- * Scratch: gs3d_linear_bwd_scratch_bytes, 16-byte aligned. */
+ * Scratch, 16-byte aligned: gs3d_linear_bwd_call_scratch_bytes of the call's own
+ * arguments (0 where it needs none, then scratch may be NULL), which depends on
+ * the sizes, the type, whether there is an activation and which gradients are
+ * not NULL; gs3d_linear_bwd_scratch_bytes is enough for every call of the sizes. */
 typedef struct gs3d_linear_bwd_args {
     int64_t rows;
     int32_t inner, outer;
@@ -605,6 +608,7 @@ typedef struct gs3d_linear_bwd_args {
 } gs3d_linear_bwd_args;
 
 size_t gs3d_linear_bwd_scratch_bytes(int64_t rows, int32_t inner, int32_t outer, int32_t dtype);
+size_t gs3d_linear_bwd_call_scratch_bytes(const gs3d_linear_bwd_args* args);
 int gs3d_linear_bwd(const gs3d_linear_bwd_args* args, void* scratch, size_t scratch_bytes, void* stream);
 
 /* y = act((x - mean) rstd weight + bias) over images of `pixels` rows each,

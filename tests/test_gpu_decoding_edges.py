@@ -99,3 +99,20 @@ def test_quantized_values_of_any_layout():
         with pytest.raises(ValueError):
             decoding.QuantizedActivations(*args).dequantize()
             pytest.fail(f"case {i} was accepted")
+
+
+def test_backward_of_a_plain_product_reserves_no_room_for_an_activation():
+    """Without an activation dz is the upstream gradient itself: beside the
+    gradients the backward pass takes the splits' sums (512 at most of dW) and
+    the weights once more."""
+    rows, inner, outer = 200_000, 64, 512
+    x, w, b, up = _case(rows, inner, outer, torch.bfloat16)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = decoding.linear(*leaves)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(y, leaves, up)
+    torch.cuda.synchronize()
+    most = sum(g.numel() * 2 for g in grads) + 512 * (outer * inner + outer) * 4 + 2 * outer * inner + (1 << 22)
+    assert torch.cuda.max_memory_allocated() - before <= most
