@@ -24,6 +24,7 @@
 #pragma once
 
 #include "linear_fused.hpp"
+#include "xcd.hpp"
 
 namespace gs3d {
 
@@ -36,18 +37,10 @@ struct LinearRows {
     void* y;             // rows x N; EPI 1 of 16-bit types: x 2 N, the second half what the first leaves of dz
     int64_t ldy;
     int64_t rows;
-    int K, N, act, n_tiles, strips;
+    int K, N, act, n_tiles, row_blocks, strips;
     int8_t* keep_codes;  // where the rows of x are kept in 8 bits, or NULL
     uint8_t* keep_scales;
 };
-
-// Blocks b, b + 8, b + 16, ... run on one XCD: the column tiles of a range of
-// rows are dealt to one of them, whose L2 then holds x once.
-GS3D_DEV void xcd_block(const LinearRows& a, int64_t& row_block, int& n_tile) {
-    const int64_t local = blockIdx.x >> 3;
-    row_block = (local / a.n_tiles) * 8 + (blockIdx.x & 7);
-    n_tile = (int)(local % a.n_tiles);
-}
 
 template <class T, int EPI>
 constexpr bool KEEPS_LOW = EPI == 1 && SPLIT<T>;
@@ -145,12 +138,9 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT, WIDE>())) v
     __shared__ u32x4 strip_lds[4][16 * (PK > PO ? PK : PO)];
     __shared__ f32x4 bias_lds[4 * NT];
 
-    int64_t row_block;
-    int n_tile;
-    xcd_block(a, row_block, n_tile);
-    const int n0 = n_tile * 16 * NT;
-    const int64_t first = row_block * a.strips * 16;
-    if (first >= a.rows) return;
+    const Dealt at_tile = deal_block(blockIdx.x, a.row_blocks, a.n_tiles);  // the column tiles of a range of rows
+    const int n_tile = at_tile.tile, n0 = n_tile * 16 * NT;
+    const int64_t first = (int64_t)at_tile.group * a.strips * 16;
     const int64_t end = first + a.strips * 16 < a.rows ? first + a.strips * 16 : a.rows;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int r = lane & 15, q = lane >> 4;
@@ -293,12 +283,9 @@ __global__ __launch_bounds__(256, 2) void linear_rows_kernel(LinearRows a) {
     __shared__ u32x4 lds[2 * STEP > OUT ? 2 * STEP : OUT];  // the weights' two buffers, then the outputs
     __shared__ float bias_lds[16 * NT];
 
-    int64_t row_block;
-    int n_tile;
-    xcd_block(a, row_block, n_tile);
-    const int n0 = n_tile * 16 * NT;
-    const int64_t first = row_block * (64 * RS);
-    if (first >= a.rows) return;
+    const Dealt at_tile = deal_block(blockIdx.x, a.row_blocks, a.n_tiles);
+    const int n0 = at_tile.tile * 16 * NT;
+    const int64_t first = (int64_t)at_tile.group * (64 * RS);
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int r = lane & 15, q = lane >> 4;
     const T* w = static_cast<const T*>(a.w);
@@ -644,11 +631,8 @@ __global__ __launch_bounds__(256, 2) void linear_gradw_kernel(LinearGradW a) {
     __shared__ u32x4 z_lds[PLANES][MR * PZ];
     __shared__ u32x4 x_lds[MR * PX];
 
-    // A split's tiles run on one XCD, whose L2 then holds its rows once.
-    const int local = blockIdx.x >> 3, tiles = a.n_tiles * a.k_tiles;
-    const int split = local / tiles * 8 + (blockIdx.x & 7);
-    if (split >= a.splits) return;
-    const int kt = local % tiles % a.k_tiles, nt = local % tiles / a.k_tiles;
+    const Dealt at_tile = deal_block(blockIdx.x, a.splits, a.n_tiles * a.k_tiles);
+    const int split = at_tile.group, kt = at_tile.tile % a.k_tiles, nt = at_tile.tile / a.k_tiles;
     const int n0 = nt * 32 * A, k0 = kt * 32 * B;
     const int64_t begin = split * a.rows_per_split;
     const int64_t end = begin + a.rows_per_split < a.rows ? begin + a.rows_per_split : a.rows;
@@ -798,17 +782,16 @@ static void launch_stream_as(LinearRows a, hipStream_t stream) {
     // blocks a compute unit: a block reads its weights once.
     int64_t strips = a.rows * a.n_tiles / (16 * 2048) / 4 * 4;
     a.strips = (int)(strips < 4 ? 4 : strips > 32 ? 32 : strips);
-    const int64_t row_blocks = (a.rows + 16 * a.strips - 1) / (16 * a.strips);
-    const int64_t blocks = (row_blocks + 7) / 8 * 8 * a.n_tiles;
-    hipLaunchKernelGGL((linear_stream_kernel<T, Q8, EPI, KCH, NT, WIDE>), dim3((unsigned)blocks), dim3(256), 0, stream,
-                       a);
+    a.row_blocks = (int)((a.rows + 16 * a.strips - 1) / (16 * a.strips));
+    hipLaunchKernelGGL((linear_stream_kernel<T, Q8, EPI, KCH, NT, WIDE>), dim3((unsigned)a.row_blocks * a.n_tiles),
+                       dim3(256), 0, stream, a);
 }
 template <class T, bool Q8, int EPI, int RS, int NT, bool WIDE>
 static void launch_long_as(LinearRows a, hipStream_t stream) {
     a.n_tiles = (a.N + 16 * NT - 1) / (16 * NT);
-    const int64_t row_blocks = (a.rows + 64 * RS - 1) / (64 * RS);
-    const int64_t blocks = (row_blocks + 7) / 8 * 8 * a.n_tiles;
-    hipLaunchKernelGGL((linear_rows_kernel<T, Q8, EPI, RS, NT, WIDE>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    a.row_blocks = (int)((a.rows + 64 * RS - 1) / (64 * RS));
+    hipLaunchKernelGGL((linear_rows_kernel<T, Q8, EPI, RS, NT, WIDE>), dim3((unsigned)a.row_blocks * a.n_tiles),
+                       dim3(256), 0, stream, a);
 }
 
 // Few rows: narrow column tiles, so that many compute units read the weights
@@ -885,7 +868,7 @@ static void launch_rows(LinearRows a, void* packed, hipStream_t stream, int time
 
 template <class T, bool Q8, int A, int B>
 static void launch_gradw_as(const LinearGradW& a, int splits, hipStream_t stream) {
-    const dim3 grid((unsigned)(a.n_tiles * a.k_tiles * ((splits + 7) / 8 * 8)));
+    const dim3 grid((unsigned)(a.n_tiles * a.k_tiles * splits));
     if constexpr (SPLIT<T>) {
         if (a.split) {
             hipLaunchKernelGGL((linear_gradw_kernel<T, Q8, A, B, 2>), grid, dim3(256), 0, stream, a);
