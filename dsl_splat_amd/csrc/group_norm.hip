@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormShape s, Rows a, No
             if constexpr (KEEP) q8_keep<T>(v, codes, scales, base + at, t.at, s.channels, true);
 #pragma unroll
             for (int i = 0; i < E; ++i) v[i] = __builtin_fmaf(v[i] - mean[i], scale[i], beta[i]);
-            activate(v, s.act);
+            activate<T>(v, s.act);
             store_row(y + (base + at) * s.channels, t.at, s.channels, pack<T>(v));
         }
     }
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(256, 4) void norm_sums_kernel(NormShape s, Rows a, 
                     v[i] -= mean[i];
                     u[i] = __builtin_fmaf(v[i], scale[i], beta[i]);
                 }
-                pull_back(g, u, s.act);
+                pull_back<T>(g, u, s.act);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     s1[i] += g[i];
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256, 4) void norm_grad_kernel(NormShape s, Rows a, 
                 v[i] -= mean[i];
                 u[i] = __builtin_fmaf(v[i], scale[i], beta[i]);
             }
-            pull_back(g, u, s.act);
+            pull_back<T>(g, u, s.act);
 #pragma unroll
             for (int i = 0; i < E; ++i)
                 v[i] = __builtin_fmaf(-v[i], along[i], __builtin_fmaf(scale[i], g[i], -level[i]));

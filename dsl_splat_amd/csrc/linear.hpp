@@ -51,13 +51,13 @@ GS3D_DEV u32x4 linear_end(const LinearRows& a, float (&z)[E], u32x4 raw_other, u
     float o[E];
     if constexpr (EPI != 0) unpack<T>(raw_other, o);
     if constexpr (EPI == 1) {
-        pull_back(o, z, a.act);
+        pull_back<T>(o, z, a.act);
         if constexpr (!SPLIT<T>) return pack<T>(o);
         const u32x4 high = take_high<T>(o);
         low = pack<T>(o);
         return high;
     } else {
-        activate(z, a.act);
+        activate<T>(z, a.act);
         if constexpr (EPI == 2) {
 #pragma unroll
             for (int i = 0; i < E; ++i) z[i] += o[i];

@@ -198,7 +198,7 @@ void linear_bwd_fused_kernel(LinearFused a) {
                     unpack<T>(z_lds[0][at], grad);
 #pragma unroll
                     for (int i = 0; i < E; ++i) arg[i] = z[i / 4][i & 3];
-                    pull_back(grad, arg, a.act);
+                    pull_back<T>(grad, arg, a.act);
                     // Past N and past the last row an infinity of x or of W
                     // meets a zero, and the slope there is NaN.
                     if (g * KC + KC > a.N || m0 + ROWS > end) {

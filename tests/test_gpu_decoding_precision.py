@@ -57,3 +57,45 @@ def test_gradients_beyond_the_range_of_float16(kind, inner, outer):
     grads = ref.linear_grads(x.detach(), w.detach(), b, up, kind)
     for name, value in zip(("x", "weight"), got):
         ref.check(name, value, *grads[name])
+
+
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+@pytest.mark.parametrize("spread", (0.5, 2.0, 8.0))
+def test_float_activations_are_as_exact_as_elementary_operations(kind, spread):
+    """z passes through a product with one weight of 1, so the error is the
+    activation's: in norm no more than half again what torch's exp, erf and
+    divisions in 32 bits leave."""
+    print(kind, spread, flush=True)
+    g = torch.Generator().manual_seed(7)
+    z = _normal(g, 1 << 18, 1, scale=spread)
+    one = torch.ones((1, 1), device=DEV)
+    leaf = z.detach().requires_grad_(True)
+    y = decoding.linear(leaf, one, activation=kind)
+    (dz,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    if kind == "silu":
+        s = torch.sigmoid(z)
+        plain = z * s, s * (1 + z * (1 - s))
+    else:
+        p = 0.5 * (1 + torch.erf(z * 0.5 ** 0.5))
+        plain = z * p, p + z * torch.exp(-0.5 * z * z) * (2 * torch.pi) ** -0.5
+    exact = ref.activate(z.double(), kind), ref.slope(z.double(), kind)
+    for name, got, other, want in zip(("value", "slope"), (y.detach(), dz), plain, exact):
+        mine, theirs = (got.double() - want).norm().item(), (other.double() - want).norm().item()
+        print(name, mine / want.norm().item(), theirs / want.norm().item(), flush=True)
+        assert mine <= 1.5 * theirs, (name, mine, theirs)
+
+
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+def test_float_activations_at_their_ends(kind):
+    """Far arguments: z or 0, slopes 1 or 0, what is not finite as by the formula."""
+    inf, nan = float("inf"), float("nan")
+    z = torch.tensor([0.0, -0.0, 90.0, -90.0, 300.0, -300.0, 1e19, -1e19, 3e38, -3e38, inf, nan], device=DEV)[:, None]
+    one = torch.ones((1, 1), device=DEV)
+    leaf = z.detach().requires_grad_(True)
+    y = decoding.linear(leaf, one, activation=kind)
+    (dz,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    y, dz = y.detach().flatten(), dz.flatten()
+    assert torch.equal(y[2:10:2], z[2:10:2, 0]) and (y[3:10:2].abs() < 1e-30).all() and not y[:2].any()
+    assert torch.equal(dz[:2], torch.full((2,), 0.5, device=DEV))
+    assert torch.equal(dz[2:10:2], torch.ones(4, device=DEV)) and (dz[3:10:2].abs() < 1e-30).all()
+    assert y[10] == inf and y[11].isnan() and dz[11].isnan()
