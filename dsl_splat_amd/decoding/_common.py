@@ -66,10 +66,18 @@ def scratch(nbytes: int, device: torch.device) -> Tensor:
 def recorded(*tensors: Tensor | None) -> bool:
     """Whether autograd has to see a call on these tensors.  One that it need
     not see runs without a node (10 us rather than 15 of host time); within
-    forward-mode differentiation all are shown, and refused by the node."""
-    if getattr(forward_ad, "_current_level", 0) >= 0:
+    forward-mode differentiation all are shown, and refused by the node, and a
+    trace keeps the node where it would keep nothing of a launch."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 or torch.jit.is_tracing():
         return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def check_untraced(name: str) -> None:
+    """RuntimeError while torch.jit.trace records: it would keep an operator
+    without a node as an uninitialised tensor."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{name} cannot be traced")
 
 
 def launch(name: str, args, device: torch.device, *rest) -> None:

@@ -8,7 +8,7 @@ import torch
 from torch import Tensor
 
 from ..runtime import native
-from ._common import DTYPES, check_input, launch, rows_of
+from ._common import DTYPES, check_input, check_untraced, launch, rows_of
 
 BLOCK = 32
 
@@ -26,6 +26,7 @@ class QuantizedActivations:
     @native.no_grad
     def dequantize(self) -> Tensor:
         """The values that were kept, in the dtype that was quantised."""
+        check_untraced("dequantize")
         codes, scales = self.codes, self.scales
         if not (isinstance(codes, Tensor) and codes.is_cuda and codes.dtype == torch.int8 and codes.ndim):
             raise ValueError("codes must be a CUDA int8 tensor of at least one dimension")
@@ -62,6 +63,7 @@ def quantize_activations(x: Tensor) -> QuantizedActivations:
     codes are rounded to nearest, ties to even, and at most 127 in size, so the
     last percent of the type's range is cut off.  Not differentiable; ``linear`` and
     ``group_norm`` keep their inputs in this form with checkpoint="int8"."""
+    check_untraced("quantize_activations")
     check_input("x", x, 1)
     x = x.detach()
     channels = x.shape[-1]

@@ -116,3 +116,27 @@ def test_backward_of_a_plain_product_reserves_no_room_for_an_activation():
     torch.cuda.synchronize()
     most = sum(g.numel() * 2 for g in grads) + 512 * (outer * inner + outer) * 4 + 2 * outer * inner + (1 << 22)
     assert torch.cuda.max_memory_allocated() - before <= most
+
+
+class _Net(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.decoder = decoding.FeatureDecoder(16, 24, 10, groups=4, device=DEV)
+
+    def forward(self, x):
+        return self.decoder(x)
+
+
+def test_traces_replay_the_operators():
+    g = torch.Generator().manual_seed(3)
+    x, other = (torch.randn((6, 7, 16), generator=g).to(DEV) for _ in range(2))
+    net = _Net()
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            traced = torch.jit.trace(net, x, check_trace=False)
+            junk = [torch.full((n,), math.nan, device=DEV) for n in (420, 1008, 4096)]  # memory that a replay may be given
+            del junk
+            for value in (other, x):
+                assert torch.equal(traced(value), net(value))
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda t: decoding.quantize_activations(t).dequantize(), x, check_trace=False)
