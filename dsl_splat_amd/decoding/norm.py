@@ -105,8 +105,8 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
         raise ValueError(f"x has more than {abi.MAX_IMAGES} images")
     check_like("weight", weight, x, (channels,))
     check_like("bias", bias, x, (channels,))
-    if isinstance(eps, bool) or not isinstance(eps, Real) or not 0.0 < eps < math.inf:
-        raise ValueError(f"eps must be positive and finite, got {eps!r}")
+    if isinstance(eps, bool) or not isinstance(eps, Real) or not 0.0 < ctypes.c_float(eps).value < math.inf:
+        raise ValueError(f"eps must be positive and finite in 32 bits, got {eps!r}")
     code = activation_code(activation)
     check_checkpoint(checkpoint)
     if not recorded(x, weight, bias):

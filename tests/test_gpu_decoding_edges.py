@@ -140,3 +140,10 @@ def test_traces_replay_the_operators():
                 assert torch.equal(traced(value), net(value))
     with pytest.raises(RuntimeError, match="trace"):
         torch.jit.trace(lambda t: decoding.quantize_activations(t).dequantize(), x, check_trace=False)
+
+
+@pytest.mark.parametrize("eps", (1e-46, 1e39))
+def test_eps_outside_32_bits_is_refused(eps):
+    """The kernels hold eps in 32 bits, where these are 0 and infinite."""
+    with pytest.raises(ValueError, match="eps"):
+        decoding.group_norm(torch.zeros((2, 2, 8), device=DEV), 2, eps=eps)
