@@ -98,13 +98,27 @@ GS3D_DEV void store_strip(const u32x4* strip, T* y, int64_t ldy, int64_t first, 
     wave_fence();
 }
 
-// Wavefronts a SIMD that the stream kernel's registers leave room for.
+// What the stream kernel keeps in LDS: 16-byte vectors of an input row and of an
+// output row, their pitches, and the vectors of a strip, of all.
+template <class T, int KCH, int NT>
+struct StreamShape {
+    static constexpr int PAD = sizeof(T) == 4 ? 1 : 2;
+    static constexpr int VK = KCH * 4, PK = VK + PAD;
+    static constexpr int VP = 16 * NT / VEC<T>, PO = VP + PAD;
+    static constexpr int STRIP = 16 * (PK > PO ? PK : PO);
+    static constexpr int LDS = KCH * NT * 64 + 4 * STRIP + 4 * NT;
+};
+
+// Wavefronts a SIMD that the stream kernel's registers and LDS leave room for (a
+// block puts one on each).
 template <class T, bool Q8, int EPI, int KCH, int NT, bool WIDE>
 constexpr int stream_waves() {
     const int wide = sizeof(T) == 4 ? 2 : 1;  // float holds twice the vectors
     const int vectors =
         wide * (2 * KCH + (EPI != 0 ? NT / 2 : 0)) + (KEEPS_LOW<T, EPI> ? NT / 2 + 1 : 0) + (WIDE ? 0 : 5);
-    return vectors <= 4 ? 6 : vectors <= 8 ? 5 : vectors <= 12 ? 4 : vectors <= 16 ? 3 : 2;
+    const int waves = vectors <= 4 ? 6 : vectors <= 8 ? 5 : vectors <= 12 ? 4 : vectors <= 16 ? 3 : 2;
+    const int blocks = 163840 / (16 * StreamShape<T, KCH, NT>::LDS);
+    return waves < blocks ? waves : blocks;
 }
 
 // A block of 4 wavefronts holds the weights of 16 NT columns in LDS, in
@@ -130,12 +144,11 @@ __global__ __launch_bounds__(256, (stream_waves<T, Q8, EPI, KCH, NT, WIDE>())) v
     constexpr int KC = CHUNK<T>;
     constexpr int TG = KC / 16;  // tiles of a lane's 16-byte output vector
     constexpr int G = NT / TG;
-    constexpr int PAD = sizeof(T) == 4 ? 1 : 2;
-    constexpr int VK = KCH * 4, PK = VK + PAD;      // an input row's vectors, and its pitch in LDS
-    constexpr int VP = 16 * NT / E, PO = VP + PAD;  // an output row's
+    using S = StreamShape<T, KCH, NT>;
+    constexpr int VK = S::VK, PK = S::PK, VP = S::VP, PO = S::PO;
     constexpr int LK = 16 * VK / 64, LP = 16 * VP / 64;
     __shared__ u32x4 w_lds[KCH * NT * 64];
-    __shared__ u32x4 strip_lds[4][16 * (PK > PO ? PK : PO)];
+    __shared__ u32x4 strip_lds[4][S::STRIP];
     __shared__ f32x4 bias_lds[4 * NT];
 
     const Dealt at_tile = deal_block(blockIdx.x, a.row_blocks, a.n_tiles);  // the column tiles of a range of rows
