@@ -808,9 +808,11 @@ static void launch_long_as(LinearRows a, hipStream_t stream) {
 }
 
 // Few rows: narrow column tiles, so that many compute units read the weights
-// at once (one row, 32 to 512 channels of float: 2.9 us, in wide tiles 6.1; 1000
-// rows, 512 to 512 of bfloat16: 7.0 and 12.6).
-static bool few_rows(const LinearRows& a) { return a.rows <= 1024; }
+// at once.  Narrow and wide (us, bfloat16): 300 rows, 512 to 512 channels 6.2
+// and 18.2; 4096 rows 13.3 and 19.2, 32 to 512 3.8 and 4.3, 256 to 64 4.1 and
+// 8.3, float 512 to 512 25.7 and 43.0; 8192 rows 24.3 and 19.5, 5.5 and 5.3, 4.3
+// and 8.5, 48.0 and 44.9.
+static bool few_rows(const LinearRows& a) { return a.rows <= 4096; }
 
 // The tile's width: 128 columns read a row once, 64 leave a float tile's LDS
 // room for twice the wavefronts (1.44 M rows of float, 32 to 128 channels: 224
@@ -827,14 +829,22 @@ static void launch_stream(const LinearRows& a, hipStream_t stream) {
     else launch_stream_as<T, Q8, EPI, KCH, MOST, true>(a, stream);
 }
 // Products that the tile kernel takes: of 16-bit types, more than 4 chunks of K,
-// as many as a block's rows find room for, and enough rows to fill the blocks.
-// It and the rows kernel in its place (us, packing included): 268177 rows, 256
-// to 512 channels of bfloat16, the forward's and the backward's two products
-// 594 and 662; 1100 rows, 512 to 64: 12.8 and 14.3; 2000 rows, 256 to 256: 10.5
-// and 8.7.  Float's rows take twice the LDS: 1.44 M rows, 128 to 64: 529 and 365.
+// as many as a block's rows find room for, enough rows to fill the blocks, and
+// enough columns for all four wavefronts of one.  It and the rows kernel in its
+// place (us, packing included, bfloat16): 268177 rows, 256 to 512 channels 127
+// and 167; 200000 rows, 512 to 512 171 and 216, 512 to 129 93 and 135, 512 to 256
+// 104 and 119, 256 to 256 61 and 63, 160 to 300 66 and 59; 32768 rows 37 and 44,
+// 25 and 30, 27 and 27, 22 and 20, 23 and 19; 16384 rows 21 and 20, 13 and 15,
+// 14 and 15, 10 and 9, 12 and 9; narrower outputs, 500000 rows, 512 to 128 206
+// and 158, 1.92 M rows, 512 to 64 686 and 457.  Float's rows take twice the LDS:
+// 1.44 M rows, 128 to 64: 529 and 365.
+template <class T>
+static bool tile_rows(int64_t rows, int K) {
+    return sizeof(T) == 2 && K > 4 * CHUNK<T> && K <= 512 && rows >= 32768;
+}
 template <class T>
 static bool tiled(int64_t rows, int K, int N) {
-    return sizeof(T) == 2 && K > 4 * CHUNK<T> && K <= 512 && rows > 1024 && N >= VEC<T>;
+    return tile_rows<T>(rows, K) && N > 128;
 }
 template <class T, bool Q8, int EPI, int KCH>
 static void launch_tile(const LinearRows& a, hipStream_t stream) {
@@ -952,9 +962,10 @@ static BwdScratch bwd_scratch(int64_t rows, int K, int N, bool act, bool params,
     return s;
 }
 
+// The forward's scratch, asked for by rows and K alone.
 template <class T>
 static size_t fwd_bytes(int64_t rows, int K, int N) {
-    return tiled<T>(rows, K, N) ? (size_t)packed_vectors<T>(N, K) * 16 : 0;
+    return tile_rows<T>(rows, K) ? (size_t)packed_vectors<T>(N, K) * 16 : 0;
 }
 
 template <class T>
@@ -964,7 +975,7 @@ static int linear_fwd(const gs3d_linear_args& g, void* scratch, hipStream_t stre
     a.w = g.weight, a.bias = g.bias, a.other = g.residual, a.ldo = g.residual_stride, a.y = g.y;
     a.rows = g.rows, a.K = g.inner, a.N = g.outer, a.ldy = g.outer, a.act = g.activation;
     // The stream kernel keeps the rows as it reads them.
-    if (g.codes && !few_rows(a) && chunks_of<T>(a.K) <= 4) a.keep_codes = g.codes, a.keep_scales = g.scales;
+    if (g.codes && chunks_of<T>(a.K) <= 4) a.keep_codes = g.codes, a.keep_scales = g.scales;
     else if (g.codes) quantize_rows(g.x, g.x_stride, g.rows, g.inner, g.dtype, g.codes, g.scales, stream);
     if (g.residual) launch_rows<T, false, 2, false>(a, scratch, stream);
     else launch_rows<T, false, 0, false>(a, scratch, stream);
