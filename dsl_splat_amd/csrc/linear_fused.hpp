@@ -84,8 +84,8 @@ void linear_bwd_fused_kernel(LinearFused a) {
     constexpr bool SKIP = sizeof(T) == 4;  // matrix instructions bound float: none for what lies past K or N
     constexpr int VK = KCH * 4, VN = NCH * 4;          // vectors of a row
     constexpr int PK = VK + S::PAD, PN = VN + S::PAD;  // pitches that spread rows over the banks, read either way
-    // Vectors are dealt to threads by powers of two a row; a row of 6 or 7
-    // chunks leaves some without.
+    // Vectors are dealt to threads by powers of two a row; a row of 7 chunks
+    // leaves some without.
     constexpr int DN = NCH > 4 ? 32 : VN;
     constexpr int RB = S::RB, ROWS = S::ROWS;
     constexpr int LK = (ROWS * VK + THREADS - 1) / THREADS, LN = (ROWS * DN + THREADS - 1) / THREADS;
@@ -306,9 +306,11 @@ void linear_bwd_fused_kernel(LinearFused a) {
 
 // Widths of 16-bit types are covered by 1, 2, 4 or 8 chunks, as far as a
 // wavefront's share of dW leaves it registers: 128 x 128, 64 x 256, 256 x 64.
-// Float's chunks are half as wide, 2, 4 or 8 of K, 2, 4, 6, 7 or 8 of N: LDS
-// decides how many blocks share a compute unit (33 to 97: 78 KB at 4 x 7, two
-// blocks; 87 KB at 4 x 8, one).
+// Float's chunks are half as wide, 2, 4 or 8 of K, 2, 4, 7 or 8 of N: LDS
+// decides how many rows a block of two on a compute unit takes at a time (us at
+// 7 chunks of N and at 8: 1.44 M rows, 33 to 97 channels 672 and 757; 1 M, 64 to
+// 112 529 and 550, 100 to 96 872 and 877, 64 to 90 498 and 505; at 6 the last
+// two 915 and 498).
 template <class T>
 static int fused_chunks_k(int channels) {
     const int chunks = (channels + CHUNK<T> - 1) / CHUNK<T>;
@@ -318,7 +320,7 @@ static int fused_chunks_k(int channels) {
 template <class T>
 static int fused_chunks_n(int channels) {
     const int chunks = (channels + CHUNK<T> - 1) / CHUNK<T>;
-    if (sizeof(T) == 4) return chunks <= 2 ? 2 : chunks <= 4 ? 4 : chunks <= 6 ? 6 : chunks;
+    if (sizeof(T) == 4) return chunks <= 2 ? 2 : chunks <= 4 ? 4 : chunks <= 7 ? 7 : 8;
     return chunks <= 2 ? chunks : chunks <= 4 ? 4 : 8;
 }
 template <class T>
@@ -364,9 +366,6 @@ static void launch_fused_n(const LinearFused& a, int blocks, hipStream_t stream)
         case 2: launch_fused_as<T, Q8, KCH, 2>(a, blocks, stream); break;
         case 4:
             if constexpr (F || KCH <= 4) launch_fused_as<T, Q8, KCH, 4>(a, blocks, stream);
-            break;
-        case 6:
-            if constexpr (F) launch_fused_as<T, Q8, KCH, 6>(a, blocks, stream);
             break;
         case 7:
             if constexpr (F) launch_fused_as<T, Q8, KCH, 7>(a, blocks, stream);
