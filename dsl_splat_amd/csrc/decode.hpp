@@ -497,8 +497,10 @@ GS3D_DEV int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
 // matrix products.  Rounded once to 16 bits it makes the error of dx 1.41
 // times, that of dW and db 1.34 to 1.53 times what rounding the results alone
 // gives.  Both products take dz as two 16-bit values, high and low, and are
-// then as exact as their own rounding.  Float, and dy itself where there is no
-// activation, are one value.
+// then as exact as their own rounding (float16's grid of 2^-24 ends both).  The
+// backward of 1.92 M rows of bfloat16, 128 to 128 channels from 8 bits, takes 387
+// us with one value, 498 with the low one in dW and 505 to 519 with it in both.
+// Float, and dy itself where there is no activation, are one value.
 // ---------------------------------------------------------------------------
 template <class T>
 constexpr bool SPLIT = sizeof(T) == 2;

@@ -24,8 +24,8 @@ struct LinearFused {
 // of 8 wavefronts where their LDS fits, of 128, 64 or 32 rows at a time, whose
 // barriers leave each other's work alone; else one of 16, the weights once for
 // all of them.  Four wavefronts a SIMD either way.  Two blocks of 32 rows and
-// one of 128 (us, silu): 1.92 M rows of bfloat16, 128 to 128 channels, 599 and
-// 639; 1 M rows, 64 to 256: 355 and 407; float, 64 to 128: 692 and 773.
+// one of 128 (us, silu): 1.92 M rows of bfloat16, 128 to 128 channels, 525 and
+// 548; 1 M rows, 64 to 256: 323 and 372; float, 64 to 128: 570 and 664.
 template <class T, int KCH, int NCH, bool ACT>
 struct FusedShape {
     static constexpr int PLANES = SPLIT<T> && ACT ? 2 : 1;
@@ -63,11 +63,10 @@ struct FusedShape {
 // Bytes bound it where K and N are small (x and dy in, dx out), the vector
 // units where the slope is dear; four wavefronts a SIMD let one's loads and
 // slopes run under another's products.  1.92 M rows of bfloat16, 32 to 128
-// channels: 187 us without an activation (3.9 TB/s), 316 with gelu; 128 to 128
-// with silu from 8 bits 498; 1.44 M rows of float, 33 to 97: 656, 70 TFLOP/s of
-// 152.  As separate products instead (us, forward and backward): 128 to 128
-// 1151, here 825; float 33 to 97 1528, here 1029; 1000 rows, 64 to 64 of
-// float16 24.8, here 15.2.
+// channels: 165 us without an activation (4.5 TB/s), 297 with gelu, whose slope
+// keeps the vector units busy 80% of the time; 128 to 128 with silu from 8 bits
+// 505, vector units 55% and matrix units 31%; 1.44 M rows of float, 33 to 97: 667,
+// matrix units 61%.  As separate products instead: 745, 920 and 1066.
 template <class T, bool Q8, int KCH, int NCH, bool WIDE, bool ACT>
 __global__ __launch_bounds__((FusedShape<T, KCH, NCH, ACT>::WAVES * 64), 4)
 void linear_bwd_fused_kernel(LinearFused a) {
