@@ -32,7 +32,8 @@ def _same(name, got, want, bound):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,inner,outer", [(300, 33, 97), (133, 40, 72), (130, 16, 5), (257, 64, 64), (200, 300, 140)])
+@pytest.mark.parametrize("rows,inner,outer", [(300, 33, 97), (133, 40, 72), (130, 16, 5), (257, 64, 64),
+                                              (200, 300, 140)])
 @pytest.mark.parametrize("checkpoint", (None, "int8"))
 def test_relu_of_infinite_arguments(checkpoint, rows, inner, outer, dtype):
     """relu's slope is 1 or 0 at an infinity, so gradients stay what the formula
@@ -134,7 +135,8 @@ def test_traces_replay_the_operators():
     for grad in (False, True):
         with torch.set_grad_enabled(grad):
             traced = torch.jit.trace(net, x, check_trace=False)
-            junk = [torch.full((n,), math.nan, device=DEV) for n in (420, 1008, 4096)]  # memory that a replay may be given
+            # Memory that a replay may be given.
+            junk = [torch.full((n,), math.nan, device=DEV) for n in (420, 1008, 4096)]
             del junk
             for value in (other, x):
                 assert torch.equal(traced(value), net(value))

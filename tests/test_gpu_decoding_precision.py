@@ -48,7 +48,8 @@ def test_gradients_beyond_the_range_of_float16(kind, inner, outer):
     g = torch.Generator().manual_seed(5)
     x = _normal(g, 1200, inner, dtype=torch.float16)
     w = _normal(g, outer, inner, scale=0.01 * inner ** -0.5, dtype=torch.float16)
-    b = torch.full((outer,), {"silu": 2.4, "gelu": 1.4}[kind], dtype=torch.float16, device=DEV)  # where the slope is largest
+    # Where the slope is largest.
+    b = torch.full((outer,), {"silu": 2.4, "gelu": 1.4}[kind], dtype=torch.float16, device=DEV)
     up = torch.zeros((1200, outer), dtype=torch.float16, device=DEV)
     up[5, 3], up[5, 4], up[700, 9] = 65504.0, -65504.0, 65504.0
     x[5], x[700] = x[5] * 2 ** -5, x[700] * 2 ** -5
